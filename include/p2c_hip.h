@@ -567,6 +567,53 @@ int p2c_eval_metrics_f32(const float *heads, int ld, int xoff, int woff, const f
                          int B, int N, int K, double *out5, int64_t *match_out, uint8_t *mask_out, double *axis64_out, float *cen_out,
                          float *found_out, void *ws, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Orthogonalised updates (csrc/muon.hip).  For every matrix X_0 = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with
+ * A = X X^T (of the smaller side); coeffs_host [steps][3] = a, b, c.  Descriptors are HOST memory and are read during the call only; their
+ * pointers are device pointers.  Strides in elements; rows * cols <= 2^31.  A matrix with no rows, columns or batch entries is skipped.
+ *   p2c_newton_schulz: dst = result.  src and dst of `dtype` (0 fp32, 1 bf16, 2 fp16), arithmetic of 32-bit accuracy for all of them.  src may be dst.
+ *   p2c_muon_step_f32 (fp32, batch = 1, mom [rows][cols] contiguous): mom = momentum mom + (1 - momentum) G;
+ *     U = nesterov ? (1 - momentum) G + momentum mom : mom;  dst = decay dst - scale newton_schulz(U).
+ * The coefficients have to keep every |X| below 3.8 and the polynomial below 15 from a start of 1 (P2C_EINVAL otherwise), steps 1 ... 16, eps > 0.
+ * ws: 16-byte aligned, p2c_newton_schulz_ws_bytes of the same descriptors, no initialisation; not shared by calls that may run at the same time.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct p2c_ns_matrix {
+    const void *src;
+    float *mom;
+    void *dst;
+    long long src_rs, src_cs, src_bs;     /* row, column, batch stride of src */
+    long long dst_rs, dst_cs, dst_bs;
+    int rows, cols, batch;
+    float scale, decay;
+} p2c_ns_matrix;
+size_t p2c_newton_schulz_ws_bytes(const p2c_ns_matrix *mats_host, int n);
+int p2c_newton_schulz(const p2c_ns_matrix *mats_host, int n, int dtype, int steps, const float *coeffs_host, double eps, void *ws,
+                      size_t ws_bytes, void *stream);
+int p2c_muon_step_f32(const p2c_ns_matrix *mats_host, int n, float momentum, int nesterov, int steps, const float *coeffs_host, double eps,
+                      void *ws, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Linear layers in 8-bit integers (csrc/int8.hip): rows and output channels carry one fp32 scale each.  dtype: 0 fp32, 1 bf16, 2 fp16.
+ * Quantised rows are [M][Kp] int8 with Kp = p2c_int8_padded(K), zeros behind K; quantised weights are [p2c_int8_padded_out(N)][Kp] with zero rows
+ * behind N (wq, 16-byte aligned), sw and bias [p2c_int8_padded_out(N)] with zeros behind N.  K <= 131072, M <= 2^30.
+ *   p2c_quantize_rows: s = max |row| * (1 / 127) in fp32, q = x / s to the nearest, ties to even, of the exact quotient.  A row with an infinity or a NaN: s = NaN,
+ *     q = 0.  A row below 2^-119 throughout: s = 0, q = 0.  ldx: row stride of x in elements (the columns are contiguous).
+ *   p2c_int8_linear: out[r][n] = act((sum_k xq wq) sx[r] sw[n] + bias[n] + add[r][n]); act 0 none, 1 ReLU, 2 softplus(beta, thr); bias, add may be NULL.
+ *   p2c_int8_linear_requant (N <= 512): the same result as quantised rows out [M][ldo = p2c_int8_padded(N)], so [M]; the fp32 values never reach memory.
+ *   p2c_int8_linear_few (M <= 32, K <= 2048): x as floats of xdtype, quantised in the same launch. */
+int p2c_int8_padded(int K);
+int p2c_int8_padded_out(int N);
+int p2c_int8_few_supported(int M, int K);
+int p2c_int8_requant_supported(int N);
+int p2c_quantize_rows(const void *x, int dtype, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, void *stream);
+int p2c_dequantize_rows(const int8_t *q, const float *scale, int M, int K, int Kp, void *out, int dtype, void *stream);
+int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx, const int8_t *wq, const float *sw, const float *bias, const float *add,
+                    long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp, void *stream);
+int p2c_int8_linear_requant(const int8_t *xq, long long ldx, const float *sx, const int8_t *wq, const float *sw, const float *bias, const float *add,
+                            long long ldadd, int act, float beta, float thr, int8_t *out, int ldo, float *so, int M, int N, int K, int Kp, void *stream);
+int p2c_int8_linear_few(const void *x, int xdtype, long long ldx, const int8_t *wq, const float *sw, const float *bias, const float *add,
+                        long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

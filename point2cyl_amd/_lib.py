@@ -108,6 +108,28 @@ _SIGS = {
 }
 
 
+
+class NsMatrix(ctypes.Structure):
+    """p2c_ns_matrix of include/p2c_hip.h."""
+    _fields_ = [("src", c_p), ("mom", c_p), ("dst", c_p), ("src_rs", c_ll), ("src_cs", c_ll), ("src_bs", c_ll), ("dst_rs", c_ll), ("dst_cs", c_ll),
+                ("dst_bs", c_ll), ("rows", c_i), ("cols", c_i), ("batch", c_i), ("scale", c_f), ("decay", c_f)]
+
+
+_SIGS.update({
+    "p2c_newton_schulz": [ctypes.POINTER(NsMatrix), c_i, c_i, c_i, ctypes.POINTER(c_f), ctypes.c_double, c_p, ctypes.c_size_t, c_p],
+    "p2c_muon_step_f32": [ctypes.POINTER(NsMatrix), c_i, c_f, c_i, c_i, ctypes.POINTER(c_f), ctypes.c_double, c_p, ctypes.c_size_t, c_p],
+    "p2c_int8_padded": [c_i],
+    "p2c_int8_padded_out": [c_i],
+    "p2c_int8_few_supported": [c_i, c_i],
+    "p2c_int8_requant_supported": [c_i],
+    "p2c_quantize_rows": [c_p, c_i, c_ll, c_i, c_i, c_i, c_p, c_p, c_p],
+    "p2c_dequantize_rows": [c_p, c_p, c_i, c_i, c_i, c_p, c_i, c_p],
+    "p2c_int8_linear": [c_p, c_ll, c_p, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p],
+    "p2c_int8_linear_requant": [c_p, c_ll, c_p, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_p],
+    "p2c_int8_linear_few": [c_p, c_i, c_ll, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p],
+})
+
+
 def declared_symbols():
     """Every function name include/p2c_hip.h declares."""
     with open(HEADER) as f:
@@ -165,6 +187,8 @@ def lib():
     L.p2c_fit_fused_supported.restype = c_i
     L.p2c_extents_ws_bytes.argtypes = [c_i, c_i]
     L.p2c_extents_ws_bytes.restype = ctypes.c_size_t
+    L.p2c_newton_schulz_ws_bytes.argtypes = [ctypes.POINTER(NsMatrix), c_i]
+    L.p2c_newton_schulz_ws_bytes.restype = ctypes.c_size_t
     L.p2c_linear_big_supported.argtypes = [c_i, c_i, c_i]
     L.p2c_linear_big_supported.restype = c_i
     L.p2c_linear_big_ws_bytes.argtypes = [c_i, c_i]

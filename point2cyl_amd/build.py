@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libp2c_hip.so")
-SOURCES = ["metrics.hip", "geom.hip", "gather.hip", "gemm.hip", "gemm_big.hip", "fwd_pp.hip", "fwd_pp3.hip", "bwd_fused.hip", "bwd_fused3.hip", "bwd_pool.hip", "heads.hip", "bn.hip", "fit.hip", "assign.hip", "loss.hip", "softplus.hip"]
+SOURCES = ["metrics.hip", "geom.hip", "gather.hip", "gemm.hip", "gemm_big.hip", "fwd_pp.hip", "fwd_pp3.hip", "bwd_fused.hip", "bwd_fused3.hip", "bwd_pool.hip", "heads.hip", "bn.hip", "fit.hip", "assign.hip", "loss.hip", "softplus.hip", "muon.hip", "int8.hip"]
 # -ffp-contract=off: geom.hip reproduces the reference's rounding order (explicit fmaf only)
 # -target-feature -packed-fp32-ops: NO v_pk_{add,mul,fma}_f32 anywhere (the host pass prints "not a recognized feature", harmless).  Round 6
 #   found farthest point sampling picking wrong points in 3 - 54 % of the HIP-graph replays in which it ran on the forked stream UNDER the
@@ -54,7 +54,7 @@ def _newer(a, b):
 
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
-    deps = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "fwd_pp.h"), os.path.join(CSRC, "lsa.h"), os.path.join(CSRC, "eigh3.h"), os.path.join(HERE, "..", "include", "p2c_hip.h")]
+    deps = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "fwd_pp.h"), os.path.join(CSRC, "tile_dma.h"), os.path.join(CSRC, "lsa.h"), os.path.join(CSRC, "eigh3.h"), os.path.join(HERE, "..", "include", "p2c_hip.h")]
     objs, dirty = [], False
     procs = []
     stamp = os.path.join(OBJ, "flags.txt")                 # objects built with other options are stale whatever their age

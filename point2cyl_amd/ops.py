@@ -4,7 +4,9 @@ Everything here is plumbing: allocate outputs with torch, pass raw device pointe
 stream to libp2c_hip.so, and register backward passes with torch.autograd.  No arithmetic of the hot
 path happens in torch ops in this file.  All feature tensors are POINT-MAJOR: [rows, channels].
 """
+import ctypes
 import os
+import struct
 
 import torch
 
@@ -1541,3 +1543,230 @@ def all_losses(W, X, normals_gt, I_gt, w_normal, w_seg):
     _lib.require_device(W, X, normals_gt, I_gt)
     out3, match, mask = _AllLosses.apply(W, X, normals_gt, I_gt, w_normal, w_seg)
     return out3, match, mask.bool()
+
+
+# ------------------------------------------------------------------------------------------ orthogonalised matrices (csrc/muon.hip)
+NS_COEFFS = (3.4445, -4.7750, 2.0315)      # a, b, c of X <- a X + (b A + c A^2) X: five steps carry every singular value of (0.01, 1] to about 1
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NS_RECORD = struct.Struct("@PPPqqqqqqiiiff4x")      # p2c_ns_matrix
+assert _NS_RECORD.size == ctypes.sizeof(_lib.NsMatrix)
+
+
+def ns_coefficients(steps, coeffs):
+    """-> ctypes float [steps * 3]: one (a, b, c) for all steps, or one per step."""
+    steps = int(steps)
+    if not 1 <= steps <= 16:
+        raise ValueError("newton_schulz: steps = %d is outside 1 ... 16" % steps)
+    rows = [tuple(coeffs)] * steps if not hasattr(coeffs[0], "__len__") else [tuple(c) for c in coeffs]
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("newton_schulz: coeffs are one (a, b, c), or one for each of the %d steps" % steps)
+    top = 1.0
+    for a, b, c in rows:                   # the same bounds as csrc/muon.hip: every matrix of the iteration has to fit a scaled fp16 pair
+        x = [top * k / 256 for k in range(257)]
+        p = max(abs(v * (a + b * v * v + c * v ** 4)) for v in x)
+        q = max([abs(a)] + [abs(b * v * v + c * v ** 4) for v in x])
+        if not (p < 3.8 and q < 15.0):
+            raise ValueError("newton_schulz: the coefficients (%g, %g, %g) drive the iteration out of range (|X| up to %g)" % (a, b, c, p))
+        top = 1.01 * p
+    return (ctypes.c_float * (3 * steps))(*[v for r in rows for v in r])
+
+
+def _ns_record(src, dst):
+    """One matrix (or batch of equal ones) as a p2c_ns_matrix; the layout along which the columns are contiguous is the one the kernels read best."""
+    r, c = src.shape[-2], src.shape[-1]
+    ss, ds = src.stride(), dst.stride()
+    b, sb, db = (src.shape[0], ss[0], ds[0]) if src.dim() == 3 else (1, 0, 0)
+    if ss[-1] != 1 and ss[-2] == 1:        # a transposed view: its transpose is orthogonalised (the same numbers), the result's strides change places too
+        return _NS_RECORD.pack(src.data_ptr(), 0, dst.data_ptr(), ss[-1], ss[-2], sb, ds[-1], ds[-2], db, c, r, b, 1.0, 1.0)
+    return _NS_RECORD.pack(src.data_ptr(), 0, dst.data_ptr(), ss[-2], ss[-1], sb, ds[-2], ds[-1], db, r, c, b, 1.0, 1.0)
+
+
+def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """The orthogonalised form of a matrix (r, c), of every matrix of a batch (..., r, c), or of every matrix of a list (any shapes, one device):
+    X_0 = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T of the smaller side - all singular values are driven
+    towards 1, the singular vectors stay.  fp32, bf16 or fp16, any strides; 32-bit accuracy inside whatever the type, one rounding at the end.
+    A zero matrix gives zeros; a matrix that holds an infinity or a NaN gives NaN (others of the call are not touched).  The result is
+    contiguous and has no gradient.  Reference use: an update rule beside torch.optim.Adam (train_Point2Cyl_without_sketch.py:204)."""
+    many = not isinstance(G, torch.Tensor)
+    items = list(G) if many else [G]
+    if not items:
+        return []
+    if not eps > 0.0:
+        raise ValueError("newton_schulz: eps = %r has to be positive" % (eps,))
+    co = ns_coefficients(steps, coeffs)
+    dev = items[0].device
+    groups, outs = {}, []
+    for g in items:
+        _lib.require_device(g)
+        if g.dim() < 2 or (many and g.dim() != 2):
+            raise ValueError("newton_schulz takes matrices (r, c), batches (..., r, c) or a list of matrices, got %s" % (tuple(g.shape),))
+        if g.dtype not in _DTYPES:
+            raise TypeError("newton_schulz takes fp32, bf16 or fp16, got %s" % g.dtype)
+        if g.device != dev:
+            raise ValueError("newton_schulz: matrices on %s and %s in one call" % (dev, g.device))
+        if g.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("newton_schulz has no gradient: call it under torch.no_grad() or on a detached tensor")
+        o = torch.empty(g.shape, dtype=g.dtype, device=dev)
+        outs.append(o)
+        if g.numel():
+            src, dst = (g, o) if g.dim() == 2 else (g.reshape(-1, *g.shape[-2:]), o.view(-1, *g.shape[-2:]))
+            # (bound to `src` until the launch: reshape may have made a copy)
+            groups.setdefault(_DTYPES[g.dtype], []).append((src, _ns_record(src, dst)))
+    with torch.cuda.device(dev):
+        for dt, recs in groups.items():
+            buf = b"".join(r for _, r in recs)
+            mats = ctypes.cast(ctypes.c_char_p(buf), ctypes.POINTER(_lib.NsMatrix))
+            nb = _lib.lib().p2c_newton_schulz_ws_bytes(mats, len(recs))
+            ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
+            call("p2c_newton_schulz", mats, len(recs), dt, int(steps), co, float(eps), ptr(ws), ws.numel(), stream())
+    return outs if many else outs[0]
+
+
+# ------------------------------------------------------------------------------------------ 8-bit linear layers (csrc/int8.hip)
+class Int8Rows:
+    """Rows in 8 bits: `q` (M, K) int8 and `scale` (M,) fp32, x ~ q * scale[:, None].  `q` is a view of rows padded to a multiple of 64 bytes with
+    zeros (what the products read)."""
+    __slots__ = ("store", "scale", "q")
+
+    def __init__(self, store, scale, K):
+        self.store, self.scale, self.q = store, scale, store[:, :K]
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self, dtype=torch.float32):
+        """q * scale as (M, K) of `dtype`."""
+        if dtype not in _DTYPES:
+            raise TypeError("dequantize gives fp32, bf16 or fp16, not %s" % dtype)
+        M, K = self.q.shape
+        out = torch.empty(M, K, dtype=dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            call("p2c_dequantize_rows", ptr(self.store), ptr(self.scale), M, K, self.store.shape[1], ptr(out), _DTYPES[dtype], stream())
+        return out
+
+
+def _int8_rows_in(x, what):
+    """x as a (M, K) float matrix whose columns are contiguous."""
+    _lib.require_device(x)
+    if x.dtype not in _DTYPES:
+        raise TypeError("%s takes fp32, bf16 or fp16, got %s" % (what, x.dtype))
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("%s has no gradient: call it under torch.no_grad() or on a detached tensor" % what)
+    if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
+        raise ValueError("%s takes rows (M, K) with K of 1 ... 131072, got %s" % (what, tuple(x.shape)))
+    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.stride(0) >= 0 else x.contiguous()
+
+
+def quantize_rows(x):
+    """Rows (M, K) of fp32, bf16 or fp16 -> Int8Rows with a scale each: scale = max |row| * (1 / 127) in fp32, q = x / scale rounded to the nearest whole
+    number, ties to even (of the exact quotient).  A row that holds an infinity or a NaN has scale NaN and q = 0 (its products are NaN, the
+    other rows are not touched); a row whose magnitudes are all below 2^-119 is a row of zeros."""
+    x = _int8_rows_in(x, "quantize_rows")
+    M, K = x.shape
+    Kp = (K + 63) // 64 * 64
+    q = torch.empty(M, Kp, dtype=torch.int8, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        call("p2c_quantize_rows", ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K, M, K, Kp, ptr(q), ptr(scale), stream(),
+             nbytes=float(M) * (K * x.element_size() + Kp))
+    return Int8Rows(q, scale, K)
+
+
+class Int8Weight:
+    """A linear layer's weight (N, K) (and bias (N,) or None) for linear_int8: one scale per output channel, laid out once.  The float tensors are
+    not kept; build it again after an optimizer step."""
+
+    def __init__(self, weight, bias=None):
+        weight = weight.detach()
+        _lib.require_device(weight, bias)
+        if weight.dim() != 2:
+            raise ValueError("Int8Weight takes a (N, K) weight, got %s" % (tuple(weight.shape),))
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError("Int8Weight: bias %s does not fit the weight %s" % (tuple(bias.shape), tuple(weight.shape)))
+        w = _int8_rows_in(weight, "Int8Weight")
+        self.N, self.K = w.shape
+        if self.N < 1:
+            raise ValueError("Int8Weight takes at least one output channel")
+        dev = w.device
+        self.Kp, Np = (self.K + 63) // 64 * 64, (self.N + 255) // 256 * 256
+        self.q = torch.zeros(Np, self.Kp, dtype=torch.int8, device=dev)
+        self.scale = torch.zeros(Np, dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            call("p2c_quantize_rows", ptr(w), _DTYPES[w.dtype], w.stride(0) if self.N > 1 else self.K, self.N, self.K, self.Kp, ptr(self.q), ptr(self.scale), stream())
+        self.bias = None
+        if bias is not None:
+            self.bias = torch.zeros(Np, dtype=torch.float32, device=dev)
+            self.bias[:self.N] = bias.detach()
+
+    @property
+    def device(self):
+        return self.q.device
+
+
+_INT8_ACTS = {None: 0, "none": 0, "relu": 1, "softplus": 2}
+
+
+def linear_int8(x, w, act="none", beta=100.0, threshold=20.0, add=None, out_dtype=None, requantize=False):
+    """act((q_x . q_w^T) s_x s_w + bias (+ add)) with whole-number products: x (..., K) floats (quantised in the call, a scale per row) or Int8Rows,
+    w an Int8Weight of K inputs.  act: "none", "relu" or "softplus" (beta, threshold as torch.nn.Softplus).  add: fp32 (M, N), added in front of
+    the activation.  Returns (..., N) of out_dtype (x's own type, fp32 for Int8Rows), or with requantize Int8Rows of the 32-bit result: for up to 512
+    channels that never reaches memory, the next layer reads 8 bits.  No gradient."""
+    if not isinstance(w, Int8Weight):
+        raise TypeError("linear_int8 takes an ops.Int8Weight, got %s" % type(w).__name__)
+    if act not in _INT8_ACTS:
+        raise ValueError("linear_int8: act %r is none of none, relu, softplus" % (act,))
+    if act == "softplus" and not beta > 0.0:
+        raise ValueError("linear_int8: softplus needs beta > 0 (got %r)" % (beta,))
+    rows = x if isinstance(x, Int8Rows) else None
+    lead = None
+    if rows is None:
+        if x.dim() != 2:
+            lead = x.shape[:-1]
+            x = x.reshape(-1, x.shape[-1]) if x.dim() else x
+        x = _int8_rows_in(x, "linear_int8")
+    M, K = x.shape
+    dev = x.device
+    if requantize and lead is not None:
+        raise ValueError("linear_int8: requantize takes rows (M, K)")
+    if K != w.K or dev != w.device:
+        raise ValueError("linear_int8: rows of %d on %s do not fit a weight of %d inputs on %s" % (K, dev, w.K, w.device))
+    if requantize and out_dtype is not None:
+        raise ValueError("linear_int8: out_dtype has no meaning with requantize")
+    out_dtype = torch.float32 if requantize else out_dtype or (x.dtype if rows is None else torch.float32)
+    if out_dtype not in _DTYPES:
+        raise TypeError("linear_int8 gives fp32, bf16 or fp16, not %s" % out_dtype)
+    ldadd = 0
+    if add is not None:
+        _lib.require_device(add)
+        if add.dtype != torch.float32 or tuple(add.shape) != (M, w.N) or add.device != dev:
+            raise ValueError("linear_int8: add is fp32 (%d, %d) on %s, got %s %s on %s" % (M, w.N, dev, add.dtype, tuple(add.shape), add.device))
+        if add.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or on a detached tensor")
+        add = add if (add.stride(1) == 1 or w.N == 1) and add.stride(0) >= w.N else add.contiguous()
+        ldadd = add.stride(0) if M > 1 else w.N
+    epi = (ptr(w.q), ptr(w.scale), ptr(w.bias), ptr(add), ldadd, _INT8_ACTS[act], float(beta), float(threshold))
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        if requantize and L.p2c_int8_requant_supported(w.N):
+            rows = rows or quantize_rows(x)
+            ldo = (w.N + 63) // 64 * 64
+            q = torch.empty(M, ldo, dtype=torch.int8, device=dev)
+            so = torch.empty(M, dtype=torch.float32, device=dev)
+            call("p2c_int8_linear_requant", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(q), ldo, ptr(so), M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
+            return Int8Rows(q, so, w.N)
+        out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
+        if M == 0:
+            pass
+        elif rows is None and L.p2c_int8_few_supported(M, K):
+            call("p2c_int8_linear_few", ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K, *epi, ptr(out), w.N, _DTYPES[out_dtype], M, w.N, K, w.Kp, stream())
+        else:
+            rows = rows or quantize_rows(x)
+            call("p2c_int8_linear", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(out), w.N, _DTYPES[out_dtype], M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
+        if requantize:
+            return quantize_rows(out)
+    return out if lead is None else out.view(*lead, w.N)

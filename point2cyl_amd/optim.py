@@ -8,9 +8,11 @@ csrc/bn.hip:adam_multi_kernel with 1024-element work items (p2c_adam_multi_f32),
 graph the gradient tensors are static).  Same update rule and operation order as torch.optim.Adam (no weight decay, no amsgrad);
 `param_groups`, `zero_grad`, `state_dict` keep torch's shapes so schedules that poke `param_groups[i]["lr"]` keep working.
 """
+import ctypes
+
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import call, ptr, stream
 
 
@@ -19,8 +21,7 @@ class Adam(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
         self._tables = {}
 
-    def _table(self, gi, group):
-        ps = [p for p in group["params"] if p.grad is not None]
+    def _table(self, gi, ps):
         # the key covers every pointer the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
         # cached table would otherwise keep pointing at the old, freed moment tensors
         key = tuple((p.data_ptr(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if (st := self.state.get(p)) else (0, 0)))
@@ -65,16 +66,116 @@ class Adam(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
-            if not any(p.grad is not None for p in group["params"]):
+            ps = [p for p in group["params"] if p.grad is not None]
+            if ps:
+                self._adam(gi, ps, group["lr"], group["betas"], group["eps"])
+        return loss
+
+    def _adam(self, gi, ps, lr, betas, eps):
+        _, tab, nel, chk, n_chunks, ps = self._table(gi, ps)
+        for p in ps:
+            self.state[p]["step"] += 1
+        steps = {int(self.state[p]["step"]) for p in ps}
+        if len(steps) != 1:     # one bias correction per launch: every tensor of the group must have taken the same number of updates
+            raise RuntimeError("point2cyl_amd.optim.Adam: parameters of one group have different step counts %s (a parameter that first "
+                               "received a gradient later than the others); put it in its own param group" % sorted(steps))
+        b1, b2 = betas
+        call("p2c_adam_multi_f32", ptr(tab), ptr(nel), ptr(chk), n_chunks, float(lr), float(b1), float(b2), float(eps),
+             int(self.state[ps[0]]["step"]), stream())
+
+
+class Muon(Adam):
+    """Orthogonalised momentum for matrices, Adam for the rest.
+
+    A parameter of two or more dimensions is a matrix (its first dimension against the others: a 1x1 convolution (Co, Ci, 1, 1) is Co x Ci):
+        m <- momentum m + (1 - momentum) g;   u = (1 - momentum) g + momentum m with nesterov, else m
+        p <- (1 - lr weight_decay) p - lr s newton_schulz(u)
+    with s = 0.2 sqrt(max(rows, columns)) for adjust="rms" (an update of the size Adam's has: Adam's learning rates and schedules carry over) or
+    sqrt(max(1, rows / columns)) for "spectral".  All matrices of a parameter group go through csrc/muon.hip together: 17 launches whatever their
+    number (chunks of 24), momentum, norm, normalisation, decay and update included.  Vectors and scalars (biases, BatchNorm), and every parameter of a
+    group with use_muon=False, take Adam's rule with the group's `betas` and `adam_eps` in one launch, without decay.
+
+    fp32, contiguous; `param_groups`, `state_dict` keep torch's shapes (state: "momentum_buffer" for matrices, Adam's three for the others).  The
+    workspace is the optimizer's own: one optimizer steps on one stream at a time."""
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, ns_coeffs=ops.NS_COEFFS, eps=1e-7, adjust="rms",
+                 betas=(0.9, 0.999), adam_eps=1e-8, use_muon=True):
+        torch.optim.Optimizer.__init__(self, params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
+                                                          ns_coeffs=ns_coeffs, eps=eps, adjust=adjust, betas=betas, adam_eps=adam_eps, use_muon=use_muon))
+        self._tables, self._mats, self._ws = {}, {}, None
+        for g in self.param_groups:
+            self._check_group(g)
+
+    @staticmethod
+    def _check_group(g):
+        if not 0.0 <= g["momentum"] < 1.0:
+            raise ValueError("Muon: momentum = %r is outside [0, 1)" % (g["momentum"],))
+        if g["adjust"] not in ("rms", "spectral"):
+            raise ValueError("Muon: adjust %r is neither rms nor spectral" % (g["adjust"],))
+        if not g["eps"] > 0.0:
+            raise ValueError("Muon: eps = %r has to be positive" % (g["eps"],))
+        ops.ns_coefficients(g["ns_steps"], g["ns_coeffs"])
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        self._mats = {}
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        self._mats = {}
+        if hasattr(self, "_ws"):                   # (not during construction)
+            self._check_group(self.param_groups[-1])
+
+    def _matrices(self, gi, ps, group):
+        """Descriptors of the group's matrices, rebuilt when a pointer, the learning rate or the decay changed."""
+        for p in ps:
+            if "momentum_buffer" not in self.state[p]:
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+        lr, wd, adjust = float(group["lr"]), float(group["weight_decay"]), group["adjust"]
+        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]), *[(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps])
+        hit = self._mats.get(gi)
+        if hit is not None and hit[0] == key:
+            return hit
+        dev = ps[0].device
+        recs = []
+        for p in ps:
+            m = self.state[p]["momentum_buffer"]
+            _lib.require_device(p, p.grad, m)
+            for t in (p, p.grad, m):
+                if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != p.shape or t.device != dev:
+                    raise RuntimeError("point2cyl_amd.optim.Muon takes contiguous fp32 parameters, gradients and momenta of one device (got %s %s on %s)"
+                                       % (t.dtype, tuple(t.shape), t.device))
+            r = p.shape[0]
+            c = p.numel() // r if r else 0
+            if not p.numel():
                 continue
-            _, tab, nel, chk, n_chunks, ps = self._table(gi, group)
-            for p in ps:
-                self.state[p]["step"] += 1
-            steps = {int(self.state[p]["step"]) for p in ps}
-            if len(steps) != 1:     # one bias correction per launch: every tensor of the group must have taken the same number of updates
-                raise RuntimeError("point2cyl_amd.optim.Adam: parameters of one group have different step counts %s (a parameter that first "
-                                   "received a gradient later than the others); put it in its own param group" % sorted(steps))
-            b1, b2 = group["betas"]
-            call("p2c_adam_multi_f32", ptr(tab), ptr(nel), ptr(chk), n_chunks, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-                 int(self.state[ps[0]]["step"]), stream())
+            s = 0.2 * max(r, c) ** 0.5 if adjust == "rms" else max(1.0, r / c) ** 0.5
+            recs.append(ops._NS_RECORD.pack(p.grad.data_ptr(), m.data_ptr(), p.data_ptr(), c, 1, 0, c, 1, 0, r, c, 1, lr * s, 1.0 - lr * wd))
+        buf = ctypes.create_string_buffer(b"".join(recs), max(1, len(recs) * ops._NS_RECORD.size))
+        mats = ctypes.cast(buf, ctypes.POINTER(_lib.NsMatrix))
+        nb = _lib.lib().p2c_newton_schulz_ws_bytes(mats, len(recs)) if recs else 0
+        hit = self._mats[gi] = (key, mats, len(recs), nb, ops.ns_coefficients(group["ns_steps"], group["ns_coeffs"]), buf)
+        return hit
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            ps = [p for p in group["params"] if p.grad is not None]
+            mats = [p for p in ps if p.dim() >= 2] if group["use_muon"] else []
+            rest = [p for p in ps if p.dim() < 2] if group["use_muon"] else ps
+            if mats:
+                _lib.require_device(*mats)
+                with torch.cuda.device(mats[0].device):
+                    _, rec, n, nb, co, _ = self._matrices(gi, mats, group)
+                    if n:
+                        if self._ws is None or self._ws.numel() < nb or self._ws.device != mats[0].device:
+                            self._ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=mats[0].device)
+                        call("p2c_muon_step_f32", rec, n, float(group["momentum"]), int(bool(group["nesterov"])), int(group["ns_steps"]), co,
+                             float(group["eps"]), ptr(self._ws), self._ws.numel(), stream())
+            if rest:
+                self._adam(gi, rest, group["lr"], group["betas"], group["adam_eps"])
         return loss

@@ -1,0 +1,485 @@
+"""GPU: the dense-layer operators - Newton-Schulz orthogonalisation, the optimizer step around it, rows in 8 bits, 8-bit linear layers - against
+their definitions in 64 bits, at the sizes, strides and values where they can go wrong; then a run of them together.
+
+Tolerances.  Newton-Schulz: a step's products carry operands of 22 bits and 32-bit sums, i.e. an error of at most delta = 2^-20 of the step's
+result in the Frobenius norm (two operand roundings of 2^-23 in each of two chained products, the polynomial's cancellation of about 2, sums), and
+what a step leaves is carried on by at most a (3.4445) per later step: |O - O_64| <= delta sum_k a^(steps - k) |X_k|, computed per matrix from
+the 64-bit iterates, plus half a unit of the output type.  8-bit: the whole-number sums are exact; scaling, bias, addend and activation are at most
+six 32-bit roundings (2^-21 of the sum of magnitudes), the fast exponential and logarithm 2^-20 of the softplus' range, then half a unit of the
+output type."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+NSC = (3.4445, -4.7750, 2.0315)
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DELTA = 2.0 ** -20
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=g, device="cuda")
+
+
+def ns64(G, steps=5, co=NSC, eps=1e-7):
+    """-> (O in 64 bits, bound on |O_kernel - O|_F)"""
+    X = G.double()
+    X = X / (X.norm() + eps)
+    tall = X.shape[0] > X.shape[1]
+    X = X.t().contiguous() if tall else X
+    bound = DELTA * X.norm().item()
+    cs = [co] * steps if not hasattr(co[0], "__len__") else co
+    for a, b, c in cs:
+        A = X @ X.t().contiguous()
+        X = a * X + (b * A + c * (A @ A)) @ X
+        bound = bound * abs(a) + DELTA * X.norm().item()
+    O = X.t().contiguous() if tall else X
+    return O, bound + HALF[G.dtype] * O.norm().item()
+
+
+def check_ns(o, G, **kw):
+    ref, bound = ns64(G, **kw)
+    assert o.shape == G.shape and o.dtype == G.dtype and o.is_contiguous()
+    err = (o.double() - ref).norm().item()
+    assert err <= bound, (tuple(G.shape), G.dtype, err, bound)
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (3, 128), (64, 3), (32, 33), (33, 32), (33, 33), (32, 1000), (1000, 31), (64, 64), (65, 130), (130, 65), (128, 131),
+          (200, 1000), (1000, 200), (127, 129), (513, 257), (1024, 512), (40, 5000)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_newton_schulz_shapes_and_types(shape, dtype):
+    from point2cyl_amd import ops
+    G = (gen(1)(*shape) * 0.01).to(dtype)
+    keep = G.clone()
+    o = ops.newton_schulz(G)
+    check_ns(o, G)
+    assert torch.equal(G, keep) and torch.equal(o, ops.newton_schulz(G))            # the input stays, the same bits again
+
+
+@pytest.mark.parametrize("kind", ["lowrank", "decay", "rank1", "zero_rows"])
+@pytest.mark.parametrize("shape", [(24, 60), (128, 131), (512, 258)])
+def test_newton_schulz_spectra(kind, shape):
+    from point2cyl_amd import ops
+    r = gen(2)
+    m, n = shape
+    if kind == "lowrank":
+        G = r(m, m // 8) @ r(m // 8, n) + 1e-3 * r(m, n)
+    elif kind == "rank1":
+        G = r(m, 1) @ r(1, n)
+    elif kind == "zero_rows":
+        G = r(m, n) * (torch.arange(m, device="cuda") % 3 == 0).float()[:, None]
+    else:
+        G = r(m, n) * torch.logspace(0, -4, m, device="cuda")[:, None]
+    check_ns(ops.newton_schulz(G), G)
+
+
+@pytest.mark.parametrize("steps,co,eps", [(1, NSC, 1e-7), (16, (1.875, -1.25, 0.375), 1e-7), (6, (1.5, -0.5, 0.0), 1e-3), (3, ((3.0, -3.2, 1.2), (2.5, -2.5, 1.0), (1.875, -1.25, 0.375)), 1e-7)])
+def test_newton_schulz_coefficients(steps, co, eps):
+    from point2cyl_amd import ops
+    for shape in ((20, 50), (96, 70)):
+        G = gen(3)(*shape)
+        check_ns(ops.newton_schulz(G, steps=steps, coeffs=co, eps=eps), G, steps=steps, co=co, eps=eps)
+
+
+def test_newton_schulz_lists_batches_and_strides():
+    from point2cyl_amd import ops
+    r = gen(4)
+    Gs = [r(*s) * 10.0 ** -(i % 7) for i, s in enumerate(SHAPES + [(64, 64)] * 13 + [(5, 5)] * 9)]      # more than one launch holds, both kernels
+    for o, G in zip(ops.newton_schulz(Gs), Gs):
+        check_ns(o, G)
+    mixed = [r(40, 50), r(40, 50).bfloat16(), r(3, 9).half(), r(0, 4), r(70, 33)]
+    for o, G in zip(ops.newton_schulz(mixed), mixed):
+        if G.numel():
+            check_ns(o, G)
+    assert ops.newton_schulz(r(0, 4)).shape == (0, 4) and ops.newton_schulz(r(2, 0, 4)).shape == (2, 0, 4)
+    for shape in ((3, 2, 40, 70), (5, 9, 4), (2, 130, 64)):
+        G = r(*shape)
+        o = ops.newton_schulz(G)
+        for x, y in zip(o.reshape(-1, *shape[-2:]), G.reshape(-1, *shape[-2:])):
+            check_ns(x, y)
+    base = r(3, 200, 300)
+    for v in (base[1].t(), base[0, ::2, ::3], base[0, 1:, 1:], base[2].t()[5:100], base[:, 10:50, 7:90], base.transpose(1, 2)[:, :60, :40], base[0].expand(2, 200, 300)):
+        o = ops.newton_schulz(v)
+        for x, y in zip(o.reshape(-1, *v.shape[-2:]), v.reshape(-1, *v.shape[-2:])):
+            check_ns(x, y)
+
+
+def test_newton_schulz_values():
+    from point2cyl_amd import ops
+    r = gen(5)
+    for shape in ((20, 30), (80, 90)):
+        assert torch.equal(ops.newton_schulz(torch.zeros(*shape, device="cuda")), torch.zeros(*shape, device="cuda"))
+        G = r(*shape)
+        for s in (1e-30, 1e30):                       # sums of squares far outside fp32
+            check_ns(ops.newton_schulz(G * s, eps=1e-38), G * s, eps=1e-38)
+        B = r(3, *shape)
+        want = ops.newton_schulz(B)
+        for bad in (float("nan"), float("inf")):
+            C = B.clone()
+            C[1, 3, 4] = bad
+            o = ops.newton_schulz(C)
+            assert torch.isnan(o[1]).all() and torch.equal(o[0], want[0]) and torch.equal(o[2], want[2])
+
+
+def test_newton_schulz_refusals():
+    from point2cyl_amd import ops
+    G = torch.ones(4, 4, device="cuda")
+    for f, e in ((lambda: ops.newton_schulz(G[0]), ValueError), (lambda: ops.newton_schulz(G.double()), TypeError), (lambda: ops.newton_schulz(G.long()), TypeError),
+                 (lambda: ops.newton_schulz(G, eps=0.0), ValueError), (lambda: ops.newton_schulz(G, steps=0), ValueError),
+                 (lambda: ops.newton_schulz([G, G[None]]), ValueError), (lambda: ops.newton_schulz([G, G.cpu()]), RuntimeError),
+                 (lambda: ops.newton_schulz(G.requires_grad_()), RuntimeError)):
+        with pytest.raises(e):
+            f()
+    with torch.no_grad():
+        ops.newton_schulz(G)
+
+
+# ------------------------------------------------------------------------------------------ Muon
+class Muon64:
+    """The update rule in 64 bits; matrices only."""
+
+    def __init__(self, ps, lr, mu, nesterov, wd, adjust):
+        self.p = [p.detach().double() for p in ps]
+        self.m = [torch.zeros_like(p) for p in self.p]
+        self.tol = [0.0] * len(ps)
+        self.lr, self.mu, self.nesterov, self.wd, self.adjust = lr, mu, nesterov, wd, adjust
+
+    def step(self, grads):
+        for i, g in enumerate(grads):
+            g = g.double()
+            self.m[i] = self.mu * self.m[i] + (1 - self.mu) * g
+            u = (1 - self.mu) * g + self.mu * self.m[i] if self.nesterov else self.m[i]
+            r, c = u.shape[0], u.numel() // u.shape[0]
+            s = 0.2 * max(r, c) ** 0.5 if self.adjust == "rms" else max(1.0, r / c) ** 0.5
+            o, bound = ns64(u.reshape(r, c).float())
+            # (the 32-bit u of the reference call carries the 2^-24 roundings of the momentum: inside delta)
+            self.p[i] = (1 - self.lr * self.wd) * self.p[i] - self.lr * s * o.view_as(u)
+            self.tol[i] += self.lr * s * 3 * bound + 2.0 ** -22 * self.p[i].norm().item()
+
+
+@pytest.mark.parametrize("nesterov,wd,adjust", [(True, 0.01, "rms"), (False, 0.0, "spectral"), (True, 0.1, "spectral")])
+def test_muon_steps(nesterov, wd, adjust):
+    from point2cyl_amd import optim
+    r = gen(6)
+    shapes = [(64, 3, 1, 1), (64, 64, 1, 1), (128, 131, 1, 1), (3, 128), (512, 258), (1, 512), (1, 1), (40, 40, 2)]
+    ps = [torch.nn.Parameter(r(*s) * 0.1) for s in shapes]
+    vec = torch.nn.Parameter(r(77))
+    idle = torch.nn.Parameter(r(5, 5))
+    vec_ref, idle_ref = torch.nn.Parameter(vec.detach().clone()), idle.detach().clone()
+    opt = optim.Muon([*ps, vec, idle], lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=wd, adjust=adjust)
+    ref = Muon64(ps, 0.02, 0.9, nesterov, wd, adjust)
+    adam = torch.optim.Adam([vec_ref], lr=0.02)
+    for step in range(3):
+        if step == 2:                                   # a schedule changes the learning rate between steps
+            opt.param_groups[0]["lr"] = adam.param_groups[0]["lr"] = ref.lr = 0.005
+        grads = [r(*s) * 1e-3 for s in shapes]
+        for p, g in zip(ps, grads):
+            p.grad = g.clone()
+        vec.grad = r(77)
+        vec_ref.grad = vec.grad.clone()
+        opt.step()
+        adam.step()
+        ref.step(grads)
+        for p, g in zip(ps, grads):
+            assert torch.equal(p.grad, g)
+    for p, q, m, tol in zip(ps, ref.p, ref.m, ref.tol):
+        assert (p.detach().double() - q).norm().item() <= tol, p.shape
+        assert (opt.state[p]["momentum_buffer"].double() - m).norm().item() <= 3 * 2.0 ** -22 * m.norm().item()
+    torch.testing.assert_close(vec, vec_ref, rtol=1e-6, atol=1e-7)
+    assert torch.equal(idle, idle_ref) and idle not in opt.state
+
+
+def test_muon_groups_state_and_refusals():
+    from point2cyl_amd import optim
+    r = gen(7)
+    a, b = torch.nn.Parameter(r(50, 60)), torch.nn.Parameter(r(50, 60))
+    b.data.copy_(a.data)
+    # use_muon=False: Adam's rule for a matrix too
+    o1, o2 = optim.Muon([{"params": [a], "use_muon": False}], lr=1e-3), torch.optim.Adam([b], lr=1e-3)
+    for _ in range(2):
+        a.grad = r(50, 60)
+        b.grad = a.grad.clone()
+        o1.step()
+        o2.step()
+    torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-7)
+    # a restored optimizer continues bit for bit
+    p, q = torch.nn.Parameter(r(70, 90)), torch.nn.Parameter(r(33, 20))
+    opt = optim.Muon([p, q], lr=0.01)
+    grads = [(r(70, 90), r(33, 20)) for _ in range(4)]
+
+    def steps(o, ps, gs):
+        for g in gs:
+            for x, y in zip(ps, g):
+                x.grad = y.clone()
+            o.step()
+    steps(opt, [p, q], grads[:2])
+    p2, q2 = torch.nn.Parameter(p.detach().clone()), torch.nn.Parameter(q.detach().clone())
+    opt2 = optim.Muon([p2, q2], lr=0.5)
+    opt2.load_state_dict(copy.deepcopy(opt.state_dict()))          # (state_dict shares its tensors with the optimizer, as torch's does)
+    steps(opt, [p, q], grads[2:])
+    steps(opt2, [p2, q2], grads[2:])
+    assert torch.equal(p, p2) and torch.equal(q, q2)
+    for bad in (torch.nn.Parameter(r(8, 8).double()), torch.nn.Parameter(r(8, 8).t()[:4].t()[::2])):
+        bad.grad = torch.ones_like(bad)
+        with pytest.raises(RuntimeError):
+            optim.Muon([bad]).step()
+
+
+# ------------------------------------------------------------------------------------------ rows in 8 bits
+def rows64(x):
+    """(q int8, scale fp32) from the definition, quotients in 64 bits."""
+    x = x.float()
+    top = x.abs().amax(1)
+    ok = torch.isfinite(x).all(1)
+    s = top * torch.tensor(1.0 / 127.0, dtype=torch.float32, device=x.device)
+    s = torch.where(top < 2.0 ** -119, torch.zeros_like(s), s)
+    q = torch.where((ok & (s > 0))[:, None], torch.round(x.double() / torch.where(s > 0, s, 1.0)[:, None].double()), 0.0)
+    return q.to(torch.int8), torch.where(ok, s, float("nan"))
+
+
+def same_scale(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=-1.0), torch.nan_to_num(b, nan=-1.0))
+
+
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 2), (5, 63), (4, 64), (7, 65), (130, 256), (9, 257), (33, 512), (6, 1024), (5, 1283), (3, 4096), (2, 4097), (2, 20000), (0, 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_quantize_rows(M, K, dtype):
+    from point2cyl_amd import ops
+    x = (gen(8)(M, K) * torch.logspace(-3, 3, M, device="cuda")[:, None]).to(dtype)
+    r = ops.quantize_rows(x)
+    q, s = rows64(x) if M else (torch.empty(0, K, dtype=torch.int8, device="cuda"), torch.empty(0, device="cuda"))
+    assert torch.equal(r.q, q) and torch.equal(r.scale, s) and r.shape == (M, K)
+    assert not r.store[:, K:].any()
+    for t in (torch.float32, torch.bfloat16, torch.float16):
+        d = r.dequantize(t)
+        assert d.dtype == t and torch.equal(d, (q.float() * s[:, None]).to(t))
+
+
+def test_quantize_rows_values():
+    from point2cyl_amd import ops
+    K = 300
+    half = torch.arange(-127, 128, device="cuda").float()
+    rows = [torch.zeros(K), torch.full((K,), 1e-40), torch.full((K,), 2.0 ** -120), torch.full((K,), 2.0 ** -119), torch.full((K,), -3.4e38), torch.full((K,), 1e-38)]
+    x = torch.stack(rows).cuda()
+    x[5, 7] = 5e-37
+    t = torch.zeros(8, K, device="cuda")                       # exact halves and their neighbours: scale 1, 2, 1/4 and a scale with few bits
+    for i, s in enumerate((1.0, 2.0, 0.25, 1.015625)):
+        for j in range(2):
+            v = (half + 0.5) * s * (1.0 - 2.0 ** -23 if j else 1.0)
+            t[2 * i + j, :255] = v
+            t[2 * i + j, 254] = 127.0 * s
+    bad = gen(9)(4, K)
+    bad[0, 5], bad[1, 299], bad[2, 0] = float("nan"), float("inf"), -float("inf")
+    x = torch.cat([x, t, bad])
+    r = ops.quantize_rows(x)
+    q, s = rows64(x)
+    assert torch.equal(r.q, q) and same_scale(r.scale, s)
+    assert int(torch.isnan(r.scale).sum()) == 3
+    g = gen(10)(500, 700)
+    for v in (g[:, ::2], g[::3], g[7:, 3:], g.t(), g[:, 5:6], g[0].expand(6, 700), g[:, :64].bfloat16()[:, 1:]):
+        r = ops.quantize_rows(v)
+        q, s = rows64(v)
+        assert torch.equal(r.q, q) and torch.equal(r.scale, s)
+
+
+# ------------------------------------------------------------------------------------------ 8-bit linear layers
+def act64(y, act, beta=100.0, thr=20.0):
+    if act == "relu":
+        return y.clamp_min(0.0)
+    if act == "softplus":
+        return torch.where(beta * y > thr, y, torch.logaddexp(torch.zeros_like(y), beta * y) / beta)
+    return y
+
+
+def linear64(q, s, wq, ws, bias=None, add=None, act="none", beta=100.0):
+    """-> (y in 64 bits, elementwise bound without the output type's rounding)"""
+    y = q.double() @ wq.double().t().contiguous() * s.double()[:, None] * ws.double()[None]
+    mag = y.abs()
+    if bias is not None:
+        y, mag = y + bias.double(), mag + bias.double().abs()
+    if add is not None:
+        y, mag = y + add.double(), mag + add.double().abs()
+    tol = mag * 2.0 ** -21
+    if act == "softplus":
+        tol = tol + 2.0 ** -20 * (1.0 / beta) + act64(y, act, beta).abs() * 2.0 ** -21
+    return act64(y, act, beta), tol
+
+
+def check_linear(o, want, tol, dtype):
+    assert o.dtype == dtype
+    lim = tol + (want.abs() + tol) * HALF[dtype] + (2.0 ** -24 if dtype == torch.float16 else 0.0)
+    bad = (o.double() - want).abs() > lim
+    assert not bad.any(), ((o.double() - want).abs() / lim).max().item()
+
+
+LINEAR = [(1, 1, 1), (1, 512, 512), (2, 3, 5), (31, 100, 33), (32, 2048, 40), (33, 64, 64), (5, 2049, 9), (64, 65, 63), (65, 200, 256), (300, 387, 254),
+          (1000, 130, 513), (4000, 512, 512), (20000, 96, 130), (13000, 260, 1030)]
+
+
+@pytest.mark.parametrize("M,K,N", LINEAR)
+@pytest.mark.parametrize("act", ["none", "relu", "softplus"])
+@pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+def test_linear_int8(M, K, N, act, dtype, out):
+    from point2cyl_amd import ops
+    r = gen(11)
+    x, W, b = r(M, K).to(dtype), r(N, K) / K ** 0.5, r(N) * 0.1
+    w = ops.Int8Weight(W, b)
+    q, s = rows64(x)
+    wq, ws = rows64(W)
+    assert torch.equal(w.q[:N, :K], wq) and torch.equal(w.scale[:N], ws)
+    want, tol = linear64(q, s, wq, ws, b, None, act)
+    y = ops.linear_int8(x, w, act=act, out_dtype=out)
+    check_linear(y, want, tol, out)
+    y2 = ops.linear_int8(ops.quantize_rows(x), w, act=act, out_dtype=out)          # rows already in 8 bits: the same numbers
+    assert torch.equal(y, y2)
+    assert torch.equal(y, ops.linear_int8(x, w, act=act, out_dtype=out))
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 64, 8), (40, 70, 254), (129, 512, 512), (700, 254, 256), (300, 100, 257), (2000, 512, 512), (130, 512, 1), (200, 64, 600)])
+@pytest.mark.parametrize("act,with_add", [("softplus", False), ("relu", True), ("none", False)])
+def test_linear_int8_requantized(M, K, N, act, with_add):
+    from point2cyl_amd import ops
+    r = gen(12)
+    x, W, b = r(M, K), r(N, K) / K ** 0.5, r(N) * 0.1
+    add = r(M, N + 3)[:, :N] if with_add else None
+    w = ops.Int8Weight(W, b)
+    h = ops.linear_int8(x, w, act=act, add=add, requantize=True)
+    y32 = ops.linear_int8(x, w, act=act, add=add, out_dtype=torch.float32)          # the same values, kept as floats
+    want, tol = linear64(*rows64(x), *rows64(W), b, add, act)
+    check_linear(y32, want, tol, torch.float32)
+    assert h.shape == (M, N) and not h.store[:, N:].any()
+    top = y32.abs().amax(1)
+    s = top * torch.tensor(1.0 / 127.0, device="cuda")
+    assert ((h.scale - s).abs() <= 2.0 ** -20 * s + 1e-30).all()                     # the epilogues may order their roundings differently
+    back = h.q.double() * h.scale.double()[:, None]
+    assert ((back - want).abs() <= tol + h.scale.double()[:, None] * 0.5001).all()   # half a quantum
+
+
+def test_linear_int8_addend_bias_and_views():
+    from point2cyl_amd import ops
+    r = gen(13)
+    for M, K, N in ((7, 40, 30), (300, 128, 254), (1, 9, 1)):
+        W, x, add = r(N, K), r(M, K), r(M, N)
+        w0 = ops.Int8Weight(W)
+        want, tol = linear64(*rows64(x), *rows64(W), None, add, "relu")
+        check_linear(ops.linear_int8(x, w0, act="relu", add=add), want, tol, torch.float32)
+        wide, wadd = r(M, 2 * K + 1), r(N, M)
+        want, tol = linear64(*rows64(wide[:, 1:K + 1]), *rows64(W), None, wadd.t())
+        check_linear(ops.linear_int8(wide[:, 1:K + 1], w0, add=wadd.t()), want, tol, torch.float32)
+        wt = ops.Int8Weight(W.t().contiguous().t(), None)
+        assert torch.equal(wt.q, w0.q) and torch.equal(wt.scale, w0.scale)
+    x3 = r(4, 5, 40)
+    w = ops.Int8Weight(r(30, 40))
+    y = ops.linear_int8(x3, w)
+    assert y.shape == (4, 5, 30) and torch.equal(y.view(20, 30), ops.linear_int8(x3.view(20, 40), w))
+    assert ops.linear_int8(r(40), w).shape == (30,) and ops.linear_int8(r(0, 40), w).shape == (0, 30)
+    assert ops.linear_int8(r(0, 40), w, requantize=True).shape == (0, 30)
+
+
+@pytest.mark.parametrize("M", [5, 500])
+def test_linear_int8_bad_rows_stay_alone(M):
+    from point2cyl_amd import ops
+    r = gen(14)
+    x, w = r(M, 100), ops.Int8Weight(r(60, 100), r(60))
+    good = ops.linear_int8(x, w, act="softplus")
+    hgood = ops.linear_int8(x, w, act="softplus", requantize=True)
+    x[1, 3], x[3, 99], x[4] = float("nan"), -float("inf"), 0.0
+    for act in ("none", "relu", "softplus"):
+        y = ops.linear_int8(x, w, act=act)
+        assert torch.isnan(y[1]).all() and torch.isnan(y[3]).all() and torch.isfinite(y[4]).all()
+        h = ops.linear_int8(x, w, act=act, requantize=True)
+        assert torch.isnan(h.scale[[1, 3]]).all() and not h.q[[1, 3]].any()
+    y, h = ops.linear_int8(x, w, act="softplus"), ops.linear_int8(x, w, act="softplus", requantize=True)
+    rest = [0, 2] + list(range(5, M))
+    assert torch.equal(y[rest], good[rest]) and torch.equal(h.q[rest], hgood.q[rest]) and torch.equal(h.scale[rest], hgood.scale[rest])
+
+
+def test_linear_int8_leaves_what_is_behind_the_rows():
+    """The C entries write M rows of N values (M rows of ldo bytes) and nothing behind them."""
+    from point2cyl_amd import _lib, ops
+    from point2cyl_amd._lib import call, ptr, stream
+    r = gen(15)
+    for M, K, N in ((3, 40, 30), (70, 130, 254), (257, 64, 300)):
+        x, w = r(M, K), ops.Int8Weight(r(N, K), r(N))
+        rows = ops.quantize_rows(x)
+        out = torch.full((M + 4, N + 5), 7.0, device="cuda")
+        call("p2c_int8_linear", ptr(rows.store), w.Kp, ptr(rows.scale), ptr(w.q), ptr(w.scale), ptr(w.bias), None, 0, 0, 1.0, 20.0, ptr(out), N + 5, 0, M, N, K, w.Kp, stream())
+        assert torch.equal(out[:M, :N], ops.linear_int8(rows, w)) and (out[M:] == 7).all() and (out[:, N:] == 7).all()
+        ldo = _lib.lib().p2c_int8_padded(N)
+        q, so = torch.full((M + 4, ldo), 7, dtype=torch.int8, device="cuda"), torch.full((M + 4,), 7.0, device="cuda")
+        call("p2c_int8_linear_requant", ptr(rows.store), w.Kp, ptr(rows.scale), ptr(w.q), ptr(w.scale), ptr(w.bias), None, 0, 0, 1.0, 20.0, ptr(q), ldo, ptr(so), M, N, K, w.Kp, stream())
+        assert (q[M:] == 7).all() and (so[M:] == 7).all() and not (q[:M, N:]).any()
+
+
+def test_int8_refusals():
+    from point2cyl_amd import ops
+    x, W = torch.ones(4, 8, device="cuda"), torch.ones(6, 8, device="cuda")
+    w = ops.Int8Weight(W)
+    for f, e in ((lambda: ops.quantize_rows(x[0]), ValueError), (lambda: ops.quantize_rows(x.double()), TypeError), (lambda: ops.quantize_rows(x[:, :0]), ValueError),
+                 (lambda: ops.quantize_rows(x.clone().requires_grad_()), RuntimeError), (lambda: ops.Int8Weight(W[0]), ValueError), (lambda: ops.Int8Weight(W[:0]), ValueError),
+                 (lambda: ops.Int8Weight(W, torch.ones(5, device="cuda")), ValueError), (lambda: ops.linear_int8(x[:, :4], w), ValueError),
+                 (lambda: ops.linear_int8(x, W), TypeError), (lambda: ops.linear_int8(x, w, act="gelu"), ValueError),
+                 (lambda: ops.linear_int8(x, w, act="softplus", beta=0.0), ValueError), (lambda: ops.linear_int8(x, w, out_dtype=torch.float64), TypeError),
+                 (lambda: ops.linear_int8(x, w, add=x), ValueError), (lambda: ops.linear_int8(x, w, requantize=True, out_dtype=torch.float32), ValueError),
+                 (lambda: ops.linear_int8(x[None], w, requantize=True), ValueError), (lambda: ops.linear_int8(x.clone().requires_grad_(), w), RuntimeError),
+                 (lambda: ops.linear_int8(x.cpu(), w), RuntimeError), (lambda: ops.quantize_rows(x).dequantize(torch.int32), TypeError)):
+        with pytest.raises(e):
+            f()
+
+
+# ------------------------------------------------------------------------------------------ streams, graphs, all together
+def test_operators_on_another_stream_and_in_a_graph():
+    from point2cyl_amd import ops, optim
+    r = gen(16)
+    Gs, x = [r(70, 90), r(20, 300), r(256, 128)], r(3000, 512)
+    w1, w2 = ops.Int8Weight(r(512, 512) / 22, r(512)), ops.Int8Weight(r(100, 512) / 22)
+    few = r(3, 512)
+
+    def run():
+        h = ops.linear_int8(x, w1, act="softplus", requantize=True)
+        return [*ops.newton_schulz(Gs), ops.linear_int8(h, w2), ops.linear_int8(few, w2)]
+    want = run()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = run()
+    st.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with torch.cuda.stream(st):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = run()
+    keep = [G.clone() for G in Gs], x.clone()
+    for k in range(4):
+        for G, G0 in zip(Gs, keep[0]):
+            G.copy_(G0 + 0.1 * k * G0.flip(0))
+        x.copy_(keep[1] * (1 + k))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(run(), out)), k
+    # an optimizer step captured: the replays advance it like eager steps
+    p, q = torch.nn.Parameter(r(70, 90)), torch.nn.Parameter(r(9, 40))
+    p2, q2 = torch.nn.Parameter(p.detach().clone()), torch.nn.Parameter(q.detach().clone())
+    for t in (p, q):
+        t.grad = r(*t.shape)
+    p2.grad, q2.grad = p.grad.clone(), q.grad.clone()
+    o, o2 = optim.Muon([p, q], lr=0.01), optim.Muon([p2, q2], lr=0.01)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        o.step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            o.step()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        o2.step()
+    assert torch.equal(p, p2) and torch.equal(q, q2)

@@ -15,10 +15,11 @@
 // Layout: X is kept twice, S = X [mP][nP] and T = X^T [nP][mP], so that all three products of a step are C[i][j] = sum_k P[i][k] Q[j][k] with
 // k contiguous: A = S S^T, B = bA + cA A^T, T' = aT + T B^T (A, B symmetric: only tiles on and above the diagonal are computed, the mirror image
 // is stored with them).  An element is 4 bytes, 8 consecutive k = 16 bytes of hi and 16 bytes of lo; sides are padded with zeros to the tile.
-// All matrices of a call go through each product together: one launch per product, whatever their number (descriptors ride in the kernel
-// arguments: no device table, capturable).  Matrices whose small side is <= 32 take ns_small_kernel: one workgroup each.
+// All matrices of a call go through each product together: one launch per product, whatever their number (the descriptors ride in the arguments of
+// the first launch: no copy from the host, capturable).  Matrices whose small side is <= 32 take ns_small: one workgroup each.
 #include "tile_dma.h"
 #include <math.h>
+#include <string.h>
 
 namespace {
 
@@ -27,9 +28,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int NS_MAX = 24;              // matrices per launch: 24 descriptors + the tile prefix stay under 4 KB of kernel arguments
-constexpr int NS_SMALL = 32;            // small sides up to here take ns_small_kernel
-constexpr int NS_SLABS = 64;            // partial sums of squares per matrix
+constexpr int NS_MAX = 24;              // matrices per chunk: the table stays under 4 KB of kernel arguments
+constexpr int NS_SMALL = 32;            // small sides up to here take ns_small
+constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at most
 constexpr float NS_SCALE = 4096.0f, NS_INV = 1.0f / 4096.0f;
 
 struct NsMat {
@@ -39,22 +40,36 @@ struct NsMat {
     int m, n, mP, nP, batch, tall;                                  // tall: the small side runs along the columns
     float scale, decay;
 };
-struct NsArgs {
+enum { NS_NORM = 0, NS_TILES = 1, NS_SYM = 2, NS_ALL = 3 };
+// The descriptors travel as an argument of the first launches; ns_begin_kernel leaves them in the workspace, with one record per workgroup of the
+// products.  A product's chain of cold misses (nothing is in the caches when a kernel starts) is then ONE long before its operands are on their way:
+// arguments preloaded into registers, record, copies.  Matrices [0, nbig) are tiled, [nbig, nbig + nsmall) small; start[phase][i]: first workgroup of
+// matrix i.
+struct NsTab {
     char *ws;
-    int nmat, dtype;                    // dtype of src and dst: 0 fp32, 1 bf16, 2 fp16
-    float mu;                           // momentum (muon)
+    int nbig, nsmall, dtype;            // dtype of src and dst: 0 fp32, 1 bf16, 2 fp16
+    float mu;                           // momentum
     int muon;                           // 0 orthogonalise, 1 momentum, 2 Nesterov momentum
     double eps;
-    int start[NS_MAX + 1];              // first workgroup of each matrix in this launch
+    int nsym, nall, tsym, tall;         // products: workgroups and tile of the symmetric ones, of the others
+    int start[4][NS_MAX + 1];
+    int small[NS_MAX + 1];
     NsMat mat[NS_MAX];
 };
+static_assert(sizeof(NsTab) % 4 == 0 && sizeof(NsTab) <= 3900, "with the coefficients within 4 KB of arguments");
 
-// workspace of one matrix: partial sums | S | T0 | T1 | A | B
+struct NsRec { unsigned long long w; int ti, tj, mP, nP, mi, b; };      // a workgroup of a product: workspace of its matrix, tile rows of P and Q
+static_assert(sizeof(NsRec) == 32, "");
+constexpr size_t NS_TAB_BYTES = (sizeof(NsTab) + 511) / 512 * 512;
+// workspace: table | records of the symmetric products, of the others | matrices
+__host__ __device__ __forceinline__ size_t ns_head(int nsym, int nall) { return NS_TAB_BYTES + ((size_t)(nsym + nall) * sizeof(NsRec) + 511) / 512 * 512; }
+
+// workspace of a matrix: partial sums | S | T0 | T1 | A | B
 __host__ __device__ __forceinline__ size_t ns_xbytes(int mP, int nP) { return (size_t)mP * nP * 4; }
-__device__ __forceinline__ char *ns_S(char *w) { return w + NS_SLABS * 8; }
-__device__ __forceinline__ char *ns_T(char *w, const NsMat &d, int which) { return ns_S(w) + (size_t)(1 + which) * ns_xbytes(d.mP, d.nP); }
-__device__ __forceinline__ char *ns_A(char *w, const NsMat &d) { return ns_S(w) + 3 * ns_xbytes(d.mP, d.nP); }
-__device__ __forceinline__ char *ns_B(char *w, const NsMat &d) { return ns_A(w, d) + ns_xbytes(d.mP, d.mP); }
+__device__ __forceinline__ char *ns_S(char *w) { return w + NS_PARTS * 8; }
+template <class D> __device__ __forceinline__ char *ns_T(char *w, const D &d, int which) { return ns_S(w) + (size_t)(1 + which) * ns_xbytes(d.mP, d.nP); }
+template <class D> __device__ __forceinline__ char *ns_A(char *w, const D &d) { return ns_S(w) + 3 * ns_xbytes(d.mP, d.nP); }
+template <class D> __device__ __forceinline__ char *ns_B(char *w, const D &d) { return ns_A(w, d) + ns_xbytes(d.mP, d.mP); }
 
 __device__ __forceinline__ float ns_get(const char *p, long long i, int dt)
 {
@@ -69,13 +84,12 @@ __device__ __forceinline__ void ns_put(char *p, long long i, int dt, float v)
     else reinterpret_cast<_Float16 *>(p)[i] = (_Float16)v;
 }
 
-// u of element (i of the small side, j of the long side); first: the momentum is advanced, else the advanced one is read
-__device__ __forceinline__ float ns_update_in(const NsArgs &a, const NsMat &d, int b, int i, int j, bool first)
+// u of row r, column c; first: the momentum is advanced, else the advanced one is read
+__device__ __forceinline__ float ns_update_in(const NsTab &a, const NsMat &d, const char *src, int r, int c, bool first)
 {
-    const long long r = d.tall ? j : i, c = d.tall ? i : j;
-    const float g = ns_get(d.src, b * d.src_bs + r * d.src_rs + c * d.src_cs, a.dtype);
+    const float g = ns_get(src, r * d.src_rs + c * d.src_cs, a.dtype);
     if (!a.muon) return g;
-    float *mp = d.mom + r * (d.tall ? d.m : d.n) + c;
+    float *mp = d.mom + (long long)r * (d.tall ? d.m : d.n) + c;
     float mv = *mp;
     if (first) {
         mv = __builtin_fmaf(a.mu, mv, (1.0f - a.mu) * g);
@@ -83,9 +97,10 @@ __device__ __forceinline__ float ns_update_in(const NsArgs &a, const NsMat &d, i
     }
     return a.muon == 2 ? __builtin_fmaf(a.mu, mv, (1.0f - a.mu) * g) : mv;
 }
+__device__ __forceinline__ const char *ns_src(const NsTab &a, const NsMat &d, int b) { return d.src + b * d.src_bs * (a.dtype == 0 ? 4 : 2); }
 
-// O's element (i, j): stored, or taken off the parameter
-__device__ __forceinline__ void ns_update_out(const NsArgs &a, const NsMat &d, int b, int i, int j, float o)
+// O's element (i of the small side, j of the long one): stored, or taken off the parameter
+__device__ __forceinline__ void ns_update_out(const NsTab &a, const NsMat &d, int b, int i, int j, float o)
 {
     const long long r = d.tall ? j : i, c = d.tall ? i : j;
     const long long at = b * d.dst_bs + r * d.dst_rs + c * d.dst_cs;
@@ -94,12 +109,21 @@ __device__ __forceinline__ void ns_update_out(const NsArgs &a, const NsMat &d, i
     *p = *p * d.decay - d.scale * o;
 }
 
-// workgroup -> (matrix, batch entry, tile of it); everything uniform
-__device__ __forceinline__ int ns_find(const NsArgs &a, int id)
+// workgroup -> matrix; everything uniform
+__device__ __forceinline__ int ns_find(const int *start, int n, int id)
 {
     int i = 0;
-    while (i + 1 < a.nmat && id >= a.start[i + 1]) ++i;
+    while (i + 1 < n && id >= start[i + 1]) ++i;
     return i;
+}
+
+// Consecutive workgroups go round the 8 XCDs; this order gives each XCD a contiguous eighth of a matrix' tiles instead, so that tiles that share
+// operand rows share an L2 (8 x 1024 x 2048: 1662 -> 1557 us a call).  Per matrix and not over the whole list: whole matrices per XCD would leave XCDs
+// with unequal work (a list of 2048 x 2048, 4000 x 1000, ...: 1579 -> 1764).
+__device__ __forceinline__ int ns_xcd_order(int id, int grid)
+{
+    const int x = id & 7, q = grid >> 3, r = grid & 7;
+    return x * q + min(x, r) + (id >> 3);
 }
 
 __device__ __forceinline__ void ns_split8(const float *v, h16x8 &hi, h16x8 &lo)
@@ -111,66 +135,40 @@ __device__ __forceinline__ void ns_split8(const float *v, h16x8 &hi, h16x8 &lo)
     }
 }
 
-// ---- sums of squares (64 bits: any 32-bit gradient fits), the momentum on the way.  NS_SLABS workgroups per matrix at most
-__global__ void __launch_bounds__(256) ns_norm_kernel(const NsArgs a)
+// 64 x 64 elements of a matrix in 16 registers a thread, 16 loads in flight: rows r0 + (tid >> 6) + 4 q, column c0 + (tid & 63)
+__device__ __forceinline__ void ns_load_tile(const NsTab &a, const NsMat &d, const char *src, int r0, int c0, bool first, float (&v)[16])
 {
-    __shared__ double red[4];
-    const int mi = ns_find(a, blockIdx.x);
+    const int rows = d.tall ? d.n : d.m, cols = d.tall ? d.m : d.n, r = r0 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v[q] = (r + 4 * q < rows && c < cols) ? ns_update_in(a, d, src, r + 4 * q, c, first) : 0.f;
+}
+
+// partial sums of a matrix: one per 64 x 64 tile of it, at most NS_PARTS
+__host__ __device__ __forceinline__ int ns_parts(int m, int n)
+{
+    const long long t = (long long)((m + 63) / 64) * ((n + 63) / 64);
+    return t < NS_PARTS ? (int)t : NS_PARTS;
+}
+
+// ---- sums of squares (64 bits: any 32-bit gradient fits), the momentum on the way
+__device__ __forceinline__ void ns_norm(const NsTab &a, int id, double *red)
+{
+    const int mi = ns_find(a.start[NS_NORM], a.nbig, id);
     const NsMat &d = a.mat[mi];
-    const int slabs = (a.start[mi + 1] - a.start[mi]) / d.batch, t = blockIdx.x - a.start[mi], b = t / slabs, slab = t - b * slabs;
-    const uint32_t total = (uint32_t)((long long)d.m * d.n), cols = d.tall ? d.m : d.n;     // at most 2^31
+    const int parts = ns_parts(d.m, d.n), t = id - a.start[NS_NORM][mi], b = t / parts, part = t - b * parts;
+    const char *src = ns_src(a, d, b);
+    const int rows = d.tall ? d.n : d.m, cols = d.tall ? d.m : d.n, tc = (cols + 63) / 64, tiles = (rows + 63) / 64 * tc;
     double s = 0.0;
-    for (uint32_t e = slab * 256 + threadIdx.x; e < total; e += slabs * 256) {
-        const int r = (int)(e / cols), c = (int)(e - r * cols);
-        const double u = ns_update_in(a, d, b, d.tall ? c : r, d.tall ? r : c, true);
-        s += u * u;
+    for (int k = part; k < tiles; k += parts) {
+        float v[16];
+        ns_load_tile(a, d, src, k / tc * 64, k % tc * 64, true, v);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) s = fma((double)v[q], (double)v[q], s);
     }
     s = p2c_wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) reinterpret_cast<double *>(a.ws + d.ws + b * d.ws_bs)[slab] = red[0] + red[1] + red[2] + red[3];
-}
-
-// ---- X_0: a 64 x 64 tile normalised and stored as S and T.  nslabs: of ns_norm_kernel's launch
-__global__ void __launch_bounds__(256) ns_begin_kernel(const NsArgs a, const int max_slabs)
-{
-    __shared__ float x[64][65];
-    __shared__ double part[NS_SLABS];
-    const int mi = ns_find(a, blockIdx.x);
-    const NsMat &d = a.mat[mi];
-    const int ti = d.mP / 64, tj = d.nP / 64, t = blockIdx.x - a.start[mi], b = t / (ti * tj), tt = t - b * (ti * tj);
-    const int i0 = tt / tj * 64, j0 = tt % tj * 64, tid = threadIdx.x;
-    char *w = a.ws + d.ws + b * d.ws_bs;
-    const int slabs = (int)min((long long)max_slabs, ((long long)d.m * d.n + 1023) / 1024);
-    if (tid < slabs) part[tid] = reinterpret_cast<const double *>(w)[tid];
-    __syncthreads();
-    double s = 0.0;
-    for (int k = 0; k < slabs; ++k) s += part[k];
-    const double inv = (double)NS_SCALE / (sqrt(s) + a.eps);
-#pragma unroll 4
-    for (int q = 0; q < 16; ++q) {
-        const int e = tid + 256 * q, u = e >> 6, v = e & 63;
-        const int i = d.tall ? v : u, j = d.tall ? u : v;
-        x[i][j] = (i0 + i < d.m && j0 + j < d.n) ? (float)((double)ns_update_in(a, d, b, i0 + i, j0 + j, false) * inv) : 0.f;
-    }
-    __syncthreads();
-    char *S = ns_S(w), *T = ns_T(w, d, 0);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int e = tid + 256 * q, r = e >> 3, c8 = (e & 7) * 8;
-        float v[8];
-        h16x8 hi, lo;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = x[r][c8 + k];
-        ns_split8(v, hi, lo);
-        h16x8 *o = reinterpret_cast<h16x8 *>(S + ((size_t)(i0 + r) * d.nP + j0 + c8) * 4);
-        o[0] = hi; o[1] = lo;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = x[c8 + k][r];
-        ns_split8(v, hi, lo);
-        o = reinterpret_cast<h16x8 *>(T + ((size_t)(j0 + r) * d.mP + i0 + c8) * 4);
-        o[0] = hi; o[1] = lo;
-    }
+    if (threadIdx.x == 0) reinterpret_cast<double *>(a.ws + d.ws + b * d.ws_bs)[part] = red[0] + red[1] + red[2] + red[3];
 }
 
 // tile t of the upper triangle of an nt x nt grid, row by row -> (i, j), j >= i
@@ -181,24 +179,86 @@ __device__ __forceinline__ void ns_triangle(int t, int nt, int &i, int &j)
     j = i + t;
 }
 
-// ---- one product of a step for every matrix.  PH 1: A = S S^T.  2: B = b A + c A A^T.  3: T' = a T + T B^T (and S').  4: as 3, into the result.
-// Tile TB x TB, four waves of TB/2 x TB/2, k-tiles of 32 (128 bytes a row) in NST LDS stages filled by direct copies, one barrier per k-tile.
-template <int TB, int NST, int PH>
-__global__ void __launch_bounds__(256) ns_product_kernel(const NsArgs a, const float ca, const float cb, const int cur)
+// table and records, spread over a launch's threads
+__device__ __forceinline__ void ns_records(const NsTab &a)
 {
-    constexpr int RB = 128, STAGE = 2 * TB * RB, NT = TB / 64, LPW = 2 * TB * RB / 1024 / 4;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    const int mi = ns_find(a, blockIdx.x);
+    if (blockIdx.x == 0)
+        for (int k = threadIdx.x; k < (int)(sizeof(NsTab) / 4); k += 256) reinterpret_cast<int *>(a.ws)[k] = reinterpret_cast<const int *>(&a)[k];
+    NsRec *rec = reinterpret_cast<NsRec *>(a.ws + NS_TAB_BYTES);
+    for (int k = blockIdx.x * 256 + threadIdx.x; k < a.nsym + a.nall; k += gridDim.x * 256) {
+        const bool sym = k < a.nsym;
+        const int id = sym ? k : k - a.nsym, *start = a.start[sym ? NS_SYM : NS_ALL], tile = sym ? a.tsym : a.tall, mi = ns_find(start, a.nbig, id);
+        const NsMat &d = a.mat[mi];
+        const int mt = d.mP / tile, per = sym ? mt * (mt + 1) / 2 : mt * (d.nP / tile);
+        int t = ns_xcd_order(id - start[mi], start[mi + 1] - start[mi]);
+        NsRec r;
+        r.mi = mi; r.mP = d.mP; r.nP = d.nP;
+        r.b = t / per;
+        t -= r.b * per;
+        if (sym) ns_triangle(t, mt, r.ti, r.tj);
+        else { r.ti = t / mt; r.tj = t - r.ti * mt; }
+        r.w = (unsigned long long)(a.ws + d.ws + r.b * d.ws_bs);
+        rec[k] = r;
+    }
+}
+
+// ---- X_0: a 64 x 64 tile normalised and stored as S and T
+__global__ void __launch_bounds__(256) ns_begin_kernel(const NsTab a)
+{
+    __shared__ float x[64][65];
+    __shared__ double red[4];
+    const int id = blockIdx.x, mi = ns_find(a.start[NS_TILES], a.nbig, id);
     const NsMat &d = a.mat[mi];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), il = lane & 31, h = lane >> 5;
-    const int mt = d.mP / TB, per = PH <= 2 ? mt * (mt + 1) / 2 : mt * (d.nP / TB);
-    int t = blockIdx.x - a.start[mi];
-    const int b = t / per;
-    t -= b * per;
-    int ti, tj;                                     // tile rows of P and of Q
-    if (PH <= 2) ns_triangle(t, mt, ti, tj);
-    else { ti = t / mt; tj = t - ti * mt; }
+    const int rows = d.tall ? d.nP : d.mP, cols = d.tall ? d.mP : d.nP, tc = cols / 64, per = rows / 64 * tc;
+    const int t = id - a.start[NS_TILES][mi], b = t / per, tt = t - b * per, r0 = tt / tc * 64, c0 = tt % tc * 64, tid = threadIdx.x;
     char *w = a.ws + d.ws + b * d.ws_bs;
+    float v[16];
+    ns_load_tile(a, d, ns_src(a, d, b), r0, c0, false, v);
+    ns_records(a);
+    const int parts = ns_parts(d.m, d.n);
+    double s = 0.0;
+    for (int k = tid; k < parts; k += 256) s += reinterpret_cast<const double *>(w)[k];
+    s = p2c_wave_sum_f64(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    const double inv = (double)NS_SCALE / (sqrt(red[0] + red[1] + red[2] + red[3]) + a.eps);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) x[(tid >> 6) + 4 * q][tid & 63] = (float)((double)v[q] * inv);
+    __syncthreads();
+    // the image whose rows are the matrix' rows, and the other
+    char *R = d.tall ? ns_T(w, d, 0) : ns_S(w), *C = d.tall ? ns_S(w) : ns_T(w, d, 0);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int e = tid + 256 * q, r = e >> 3, c8 = (e & 7) * 8;
+        float u[8];
+        h16x8 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = x[r][c8 + k];
+        ns_split8(u, hi, lo);
+        h16x8 *o = reinterpret_cast<h16x8 *>(R + ((size_t)(r0 + r) * cols + c0 + c8) * 4);
+        o[0] = hi; o[1] = lo;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = x[c8 + k][r];
+        ns_split8(u, hi, lo);
+        o = reinterpret_cast<h16x8 *>(C + ((size_t)(c0 + r) * rows + r0 + c8) * 4);
+        o[0] = hi; o[1] = lo;
+    }
+}
+
+// ---- one product of a step for every matrix.  PH 1: A = S S^T.  2: B = b A + c A A^T.  3: T' = a T + T B^T (and S').  4: as 3, into the result.
+// Tile TB x TB, one wave of 32 x 32 (TB = 32) or four waves of TB/2 x TB/2 for each of KG groups that share the k range (group g takes k-tiles
+// g, g + KG, ...); k-tiles of 32 (128 bytes a row) in NST LDS stages filled by direct copies, one barrier per KG k-tiles.
+template <int TB, int KG, int NST, int PH>
+__global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(const NsTab *__restrict__ tab, const NsRec *__restrict__ recs, const float ca, const float cb, const int cur)
+{
+    constexpr int WG = TB == 32 ? 1 : 4, RB = 128, TILE = 2 * TB * RB, STAGE = KG * TILE, NT = TB == 128 ? 2 : 1, LPW = TILE / 1024 / WG;
+    constexpr int GP = 4 / KG;                      // row groups of a piece (8 g + 4 h + 0..3) that a k-group finishes
+    static_assert(KG == 1 || NT == 1, "");
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const NsRec d = recs[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, gw = __builtin_amdgcn_readfirstlane(tid >> 6), wave = gw % WG, kg = gw / WG, il = lane & 31, h = lane >> 5;
+    const int ti = d.ti, tj = d.tj;                 // tile rows of P and of Q
+    char *w = reinterpret_cast<char *>(d.w);
     const char *P, *Q;
     int K;
     if (PH == 1) { P = Q = ns_S(w); K = d.nP; }
@@ -207,7 +267,29 @@ __global__ void __launch_bounds__(256) ns_product_kernel(const NsArgs a, const f
     const long long ld = (long long)K * 4;
     P += (long long)ti * TB * ld;
     Q += (long long)tj * TB * ld;
-    const int KT = K / 32;
+    const int KT = K / 32, IT = (KT + KG - 1) / KG;
+
+    const int wr = WG == 1 ? 0 : (wave >> 1) * (TB / 2), wc = WG == 1 ? 0 : (wave & 1) * (TB / 2);
+    const bool mirror = PH == 3 || (PH <= 2 && ti != tj);
+    char *o1 = PH == 1 ? ns_A(w, d) : PH == 2 ? ns_B(w, d) : ns_T(w, d, cur ^ 1);
+    char *o2 = PH == 3 || PH == 4 ? ns_S(w) : o1;
+    const char *old = PH == 2 ? ns_A(w, d) : ns_S(w);
+    const int ld1 = d.mP, ld2 = PH <= 2 ? d.mP : d.nP;
+    auto at2 = [&](int x, int y, int g) { return ((size_t)(tj * TB + wc + y * 32 + il) * ld2 + ti * TB + wr + x * 32 + 8 * g) * 4 + 8 * h; };
+    // the addend is fetched ahead of the operands: behind the sums it would be one more trip to memory at the kernel's end
+    h16x4 oldh[NT][NT][GP], oldl[NT][NT][GP];
+    if (PH != 1) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+#pragma unroll
+                for (int g = 0; g < GP; ++g) {
+                    const char *q = old + at2(x, y, kg * GP + g);
+                    oldh[x][y][g] = *reinterpret_cast<const h16x4 *>(q);
+                    oldl[x][y][g] = *reinterpret_cast<const h16x4 *>(q + 16);
+                }
+    }
 
     f32x16 acc[NT][NT];
 #pragma unroll
@@ -217,237 +299,353 @@ __global__ void __launch_bounds__(256) ns_product_kernel(const NsArgs a, const f
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[p][q][r] = 0.f;
 
-#define P2C_NS_COPY(KT_)                                                                             \
+#define P2C_NS_COPY(IT_)                                                                             \
     do {                                                                                             \
-        const int k__ = min((KT_), KT - 1);                                                          \
-        char *st__ = smem + ((KT_) % NST) * STAGE;                                                   \
-        p2c_tile_copy<TB, RB, 4>(P + (long long)k__ * RB, ld, TB - 1, st__, wave, lane);             \
-        p2c_tile_copy<TB, RB, 4>(Q + (long long)k__ * RB, ld, TB - 1, st__ + TB * RB, wave, lane);   \
+        const int k__ = min((IT_) * KG + kg, KT - 1);                                                \
+        char *st__ = smem + ((IT_) % NST) * STAGE + kg * TILE;                                       \
+        p2c_tile_copy<TB, RB, WG>(P + (long long)k__ * RB, ld, TB - 1, st__, wave, lane);            \
+        p2c_tile_copy<TB, RB, WG>(Q + (long long)k__ * RB, ld, TB - 1, st__ + TB * RB, wave, lane);  \
     } while (0)
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) P2C_NS_COPY(s);
-    const int wr = (wave >> 1) * (TB / 2), wc = (wave & 1) * (TB / 2);
-    for (int kt = 0; kt < KT; ++kt) {
-        p2c_tile_wait<(NST - 2) * LPW>();           // stage kt is here, and nobody reads stage kt - 1 any more
-        P2C_NS_COPY(kt + NST - 1);                  // (past the end: the last tile again, into a stage that is never read: the count in flight stays exact)
-        const char *ps = smem + (kt % NST) * STAGE, *qs = ps + TB * RB;
+    for (int it = 0; it < IT; ++it) {
+        p2c_tile_wait<(NST - 2) * LPW>();           // stage `it` is here, and nobody reads stage it - 1 any more
+        P2C_NS_COPY(it + NST - 1);                  // (past the end: the last tile again, into a stage that is never read: the count in flight stays exact)
+        if (KG > 1 && it * KG + kg >= KT) continue;
+        const char *ps = smem + (it % NST) * STAGE + kg * TILE, *qs = ps + TB * RB;
+        // every fragment of the k-tile is requested before the first product (left to itself the compiler waits for LDS three times per k-step)
+        h16x8 p[2][NT][2], q[2][NT][2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            h16x8 p[NT][2], q[NT][2];
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int x = 0; x < NT; ++x)
 #pragma unroll
                 for (int pl = 0; pl < 2; ++pl) {
                     const int c = (2 * s + h) * 2 + pl;
-                    p[x][pl] = *reinterpret_cast<const h16x8 *>(ps + p2c_tile_at<RB>(wr + x * 32 + il, c));
-                    q[x][pl] = *reinterpret_cast<const h16x8 *>(qs + p2c_tile_at<RB>(wc + x * 32 + il, c));
+                    p[s][x][pl] = *reinterpret_cast<const h16x8 *>(ps + p2c_tile_at<RB>(wr + x * 32 + il, c));
+                    q[s][x][pl] = *reinterpret_cast<const h16x8 *>(qs + p2c_tile_at<RB>(wc + x * 32 + il, c));
                 }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int pr = 0; pr < 3; ++pr)          // small products first
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
                     for (int y = 0; y < NT; ++y)
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[x][pr == 1], q[y][pr == 0], acc[x][y], 0, 0, 0);
-        }
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[s][x][pr == 1], q[s][y][pr == 0], acc[x][y], 0, 0, 0);
     }
 #undef P2C_NS_COPY
     p2c_tile_wait<0>();                             // the surplus copies have landed: the stages are free
 
     // ---- epilogue.  A lane holds column il of a 32 x 32 piece, rows 8 g + 4 h + (0..3): four consecutive k of the transposed image, which is
-    // read (the addend) and written from the registers; the straight image goes through LDS to get 8 consecutive k per lane.
-    float *stage = reinterpret_cast<float *>(smem) + wave * (32 * 36);
-    const bool mirror = PH == 3 || (PH <= 2 && ti != tj);
-    char *o1 = PH == 1 ? ns_A(w, d) : PH == 2 ? ns_B(w, d) : ns_T(w, d, cur ^ 1);
-    char *o2 = PH == 3 || PH == 4 ? ns_S(w) : o1;
-    const char *old = PH == 2 ? ns_A(w, d) : ns_S(w);
-    const int ld1 = d.mP, ld2 = PH <= 2 ? d.mP : d.nP;
+    // read (the addend) and written from the registers; the straight image goes through LDS to get consecutive k per lane.
+    // one group g of four rows of piece (x, y): c = the sums; leaves the new values in c
+    auto finish = [&](int x, int y, int g, h16x4 oh, h16x4 ol, float (&c)[4]) {
+        if (PH == 1) {
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+            for (int e = 0; e < 4; ++e) c[e] *= NS_INV;
+        } else {
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            const int r0 = ti * TB + wr + x * 32, c0 = tj * TB + wc + y * 32, col = c0 + il;
+            for (int e = 0; e < 4; ++e) c[e] = __builtin_fmaf(ca, (float)oh[e] + (float)ol[e], cb * (c[e] * NS_INV));
+        }
+        if (mirror) {
+            h16x4 vh, vl;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const size_t at2 = ((size_t)col * ld2 + r0 + 8 * g) * 4 + 8 * h;
-                float v[4];
-                if (PH == 1) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e] * NS_INV;
-                } else {
-                    const h16x4 oh = *reinterpret_cast<const h16x4 *>(old + at2), ol = *reinterpret_cast<const h16x4 *>(old + at2 + 16);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ca, (float)oh[e] + (float)ol[e], cb * (acc[x][y][4 * g + e] * NS_INV));
-                }
-                if (PH == 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = col, j = r0 + 8 * g + 4 * h + e;
-                        if (i < d.m && j < d.n) ns_update_out(a, d, b, i, j, v[e] * NS_INV);
-                    }
-                } else {
-                    if (mirror) {
-                        h16x4 vh, vl;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            vh[e] = (_Float16)v[e];
-                            vl[e] = (_Float16)(v[e] - (float)vh[e]);
-                        }
-                        *reinterpret_cast<h16x4 *>(o2 + at2) = vh;
-                        *reinterpret_cast<h16x4 *>(o2 + at2 + 16) = vl;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) stage[(8 * g + 4 * h + e) * 36 + il] = v[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                vh[e] = (_Float16)c[e];
+                vl[e] = (_Float16)(c[e] - (float)vh[e]);
             }
-            if (PH != 4) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            char *o = o2 + at2(x, y, g);
+            *reinterpret_cast<h16x4 *>(o) = vh;
+            *reinterpret_cast<h16x4 *>(o + 16) = vl;
+        }
+    };
+    // a 32 x 32 piece of the result: lanes run along the contiguous side of the output
+    constexpr int LDS_ = PH == 4 ? 33 : 36;
+    auto last = [&](const float *stage, int x, int y, int first, int count) {
+        const NsMat &m = tab->mat[d.mi];
+        const int i0 = tj * TB + wc + y * 32, j0 = ti * TB + wr + x * 32;
+#pragma unroll 4
+        for (int e = first; e < 1024; e += count) {
+            const int u = e >> 5, v = e & 31, i = m.tall ? v : u, j = m.tall ? u : v;
+            if (i0 + i < m.m && j0 + j < m.n) ns_update_out(*tab, m, d.b, i0 + i, j0 + j, stage[j * LDS_ + i] * NS_INV);
+        }
+    };
+    if (KG == 1) {
+        float *stage = reinterpret_cast<float *>(smem) + wave * (32 * 36);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int u = lane + 64 * q, r = u >> 2, c8 = (u & 3) * 8;
-                    float v[8];
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = stage[r * 36 + c8 + k];
-                    h16x8 hi, lo;
-                    ns_split8(v, hi, lo);
-                    h16x8 *o = reinterpret_cast<h16x8 *>(o1 + ((size_t)(r0 + r) * ld1 + c0 + c8) * 4);
-                    o[0] = hi; o[1] = lo;
+            for (int y = 0; y < NT; ++y) {
+                const int r0 = ti * TB + wr + x * 32, c0 = tj * TB + wc + y * 32;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float c[4] = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]};
+                    finish(x, y, g, oldh[x][y][g], oldl[x][y][g], c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) stage[(8 * g + 4 * h + e) * LDS_ + il] = c[e];
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (PH == 4) {
+                    last(stage, x, y, lane, 64);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int u = lane + 64 * q, r = u >> 2, c8 = (u & 3) * 8;
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = stage[r * LDS_ + c8 + k];
+                        h16x8 hi, lo;
+                        ns_split8(v, hi, lo);
+                        h16x8 *o = reinterpret_cast<h16x8 *>(o1 + ((size_t)(r0 + r) * ld1 + c0 + c8) * 4);
+                        o[0] = hi; o[1] = lo;
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+    } else {
+        // the groups' sums meet in LDS; group k finishes the rows 8 g + 4 h + (0..3), g = GP k ... GP k + GP - 1, of its wave's piece
+        f32x4 *sums = reinterpret_cast<f32x4 *>(smem);                               // [group][wave][g][lane]
+        float *stage = reinterpret_cast<float *>(smem + KG * WG * 4 * 64 * 16) + wave * (32 * 36);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            sums[((kg * WG + wave) * 4 + g) * 64 + lane] = f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
+        __syncthreads();
+        const int r0 = ti * TB + wr, c0 = tj * TB + wc;
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KG; ++k) {
+                const f32x4 v = sums[((k * WG + wave) * 4 + kg * GP + g) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] += v[e];
+            }
+            finish(0, 0, kg * GP + g, oldh[0][0][g], oldl[0][0][g], c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) stage[(8 * (kg * GP + g) + 4 * h + e) * LDS_ + il] = c[e];
+        }
+        __syncthreads();
+        if (PH == 4) {
+            last(stage, 0, 0, kg * 64 + lane, 64 * KG);
+        } else {
+#pragma unroll
+            for (int q = 0; q < GP; ++q) {
+                const int u = (q * KG + kg) * 64 + lane, r = u >> 3, c4 = (u & 7) * 4;      // four consecutive k per lane
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(stage + r * 36 + c4);
+                h16x4 vh, vl;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    vh[e] = (_Float16)v[e];
+                    vl[e] = (_Float16)(v[e] - (float)vh[e]);
+                }
+                char *o = o1 + ((size_t)(r0 + r) * ld1 + c0 + (c4 & ~7)) * 4 + (c4 & 4) * 2;
+                *reinterpret_cast<h16x4 *>(o) = vh;
+                *reinterpret_cast<h16x4 *>(o + 16) = vl;
             }
         }
+    }
 }
 
 // ---- small side <= 32: one workgroup per matrix, in the m x m space and in 64 bits.  X_k = Q_k X_0 with Q and A polynomials of A_0 = X_0 X_0^T:
 // q = a + bA + cA^2, Q <- q Q, A <- q A q.  G is read twice and nothing else moves.  64 bits are what this form needs (A holds SQUARED singular
 // values and a rounding grows by a^2 per step: 2.5e5 over five); at this size they cost less than the launches of the tiled form.
-// coefficients: [steps][3] in constant order a, b, c
 struct NsCoef { int steps; float c[16][3]; };
 
-__device__ __forceinline__ double ns_dot(const double (*x)[NS_SMALL + 1], const double (*y)[NS_SMALL + 1], int i, int j, int m)
+constexpr int NS_XS = 2112;                                     // floats of a chunk of X: m rows of 64 ... 2048 elements, each padded by one
+
+struct NsSmallLds {
+    double A[NS_SMALL][NS_SMALL + 1], Q[NS_SMALL][NS_SMALL + 1], U[NS_SMALL][NS_SMALL + 1], V[NS_SMALL][NS_SMALL + 1];
+    float x[NS_XS];
+};
+
+template <int M>
+__device__ __forceinline__ double ns_dot(const double (*x)[NS_SMALL + 1], const double (*y)[NS_SMALL + 1], int i, int j)
 {
     double s = 0.0;
-    for (int k = 0; k < m; ++k) s = fma(x[i][k], y[k][j], s);
+#pragma unroll 8
+    for (int k = 0; k < M; ++k) s = fma(x[i][k], y[k][j], s);
     return s;
 }
 
-__global__ void __launch_bounds__(256) ns_small_kernel(const NsArgs a, const NsCoef co)
+// M: a power of two >= m, at least 4; the matrices are padded with zeros to M.  The 2 x 2 blocks of the M x M Gram matrix take (M/2)^2 threads; the
+// others share the long side.
+template <int M>
+__device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int mi, int b, NsSmallLds &l)
 {
-    __shared__ double A[NS_SMALL][NS_SMALL + 1], Q[NS_SMALL][NS_SMALL + 1], U[NS_SMALL][NS_SMALL + 1], V[NS_SMALL][NS_SMALL + 1];
-    __shared__ float x[NS_SMALL][65];
-    const int mi = ns_find(a, blockIdx.x);
+    constexpr int BL = M / 2, SPLIT = 256 / (BL * BL), JC = 2048 / M, LDX = JC + 1, PER = (M * M + 255) / 256;
+    static_assert(M * LDX <= NS_XS && SPLIT <= JC, "");
     const NsMat &d = a.mat[mi];
-    const int b = blockIdx.x - a.start[mi], tid = threadIdx.x, m = d.m, n = d.n;
-    const int pi = tid >> 4, pj = tid & 15;                     // this thread's 2 x 2 entries of an m x m matrix
+    const int tid = threadIdx.x, m = d.m, n = d.n;
+    const int blk = tid % (BL * BL), sp = tid / (BL * BL), pi = blk / BL, pj = blk % BL;
+    const char *src = ns_src(a, d, b);
     double g[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
-    const int tasks = m * 64;
-    // 64 long indices at a time, the next ones in flight under the sums
-    float nx[8];
+    float nx[8];                                                // the next chunk, in flight under the sums of this one: 2048 elements
+    auto place_of = [&](int e, int &i, int &j) {                // wide: j runs along the lanes, tall: i does
+        if (d.tall) { i = e % M; j = e / M; } else { i = e / JC; j = e % JC; }
+    };
     auto fetch = [&](int j0, bool first) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const int e = tid + 256 * q;
-            const int i = d.tall ? e % m : e >> 6, j = j0 + (d.tall ? e / m : e & 63);
-            nx[q] = (e < tasks && j < n) ? ns_update_in(a, d, b, i, j, first) : 0.f;
+            int i, j;
+            place_of(tid + 256 * q, i, j);
+            j += j0;
+            nx[q] = (i < m && j < n) ? ns_update_in(a, d, src, d.tall ? j : i, d.tall ? i : j, first) : 0.f;
         }
     };
     auto place = [&]() {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const int e = tid + 256 * q;
-            if (e < tasks) x[d.tall ? e % m : e >> 6][d.tall ? e / m : e & 63] = nx[q];
+            int i, j;
+            place_of(tid + 256 * q, i, j);
+            l.x[i * LDX + j] = nx[q];
         }
     };
     fetch(0, true);
-    for (int j0 = 0; j0 < n; j0 += 64) {
+    for (int j0 = 0; j0 < n; j0 += JC) {
         __syncthreads();
         place();
         __syncthreads();
-        if (j0 + 64 < n) fetch(j0 + 64, true);
-        if (2 * pi < m && 2 * pj < m) {
-            const int i1 = min(2 * pi + 1, m - 1), k1 = min(2 * pj + 1, m - 1);
-#pragma unroll 4
-            for (int j = 0; j < 64; ++j) {
-                const double u0 = x[2 * pi][j], u1 = x[i1][j], v0 = x[2 * pj][j], v1 = x[k1][j];
-                g[0][0] = fma(u0, v0, g[0][0]);
-                g[0][1] = fma(u0, v1, g[0][1]);
-                g[1][0] = fma(u1, v0, g[1][0]);
-                g[1][1] = fma(u1, v1, g[1][1]);
-            }
+        if (j0 + JC < n) fetch(j0 + JC, true);
+#pragma unroll 8
+        for (int j = sp; j < JC; j += SPLIT) {
+            const double u0 = l.x[2 * pi * LDX + j], u1 = l.x[(2 * pi + 1) * LDX + j], v0 = l.x[2 * pj * LDX + j], v1 = l.x[(2 * pj + 1) * LDX + j];
+            g[0][0] = fma(u0, v0, g[0][0]);
+            g[0][1] = fma(u0, v1, g[0][1]);
+            g[1][0] = fma(u1, v0, g[1][0]);
+            g[1][1] = fma(u1, v1, g[1][1]);
         }
     }
+    if (SPLIT == 1) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
+        for (int p = 0; p < 4; ++p) l.A[2 * pi + (p >> 1)][2 * pj + (p & 1)] = g[p >> 1][p & 1];
+        __syncthreads();
+    } else {
+        double *part = &l.U[0][0];                              // [4][256], over U
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-            if (2 * pi + p < m && 2 * pj + q < m) A[2 * pi + p][2 * pj + q] = g[p][q];
-    __syncthreads();
+        for (int p = 0; p < 4; ++p) part[p * 256 + tid] = g[p >> 1][p & 1];
+        __syncthreads();
+        if (tid < M * M) {
+            const int i = tid / M, j = tid % M, p = (i & 1) * 2 + (j & 1), at = (i >> 1) * BL + (j >> 1);
+            double s = 0.0;
+#pragma unroll 8
+            for (int k = 0; k < SPLIT; ++k) s += part[p * 256 + k * BL * BL + at];
+            l.A[i][j] = s;
+        }
+        __syncthreads();
+    }
     double tr = 0.0;
-    for (int k = 0; k < m; ++k) tr += A[k][k];
+#pragma unroll
+    for (int k = 0; k < M; ++k) tr += l.A[k][k];
     const double inv = 1.0 / (sqrt(tr) + a.eps);
     __syncthreads();
-    for (int e = tid; e < m * m; e += 256) {
-        const int i = e / m, j = e - i * m;
-        A[i][j] *= inv * inv;
-        Q[i][j] = i == j ? inv : 0.0;                           // the normalisation of X_0 rides in Q
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int e = tid + 256 * q, i = e / M, j = e % M;
+        if (e < M * M) {
+            l.A[i][j] *= inv * inv;
+            l.Q[i][j] = i == j ? inv : 0.0;                     // the normalisation of X_0 rides in Q
+        }
     }
     __syncthreads();
     for (int s = 0; s < co.steps; ++s) {
         const double c0 = co.c[s][0], c1 = co.c[s][1], c2 = co.c[s][2];
-        for (int e = tid; e < m * m; e += 256) {
-            const int i = e / m, j = e - i * m;
-            U[i][j] = c2 * ns_dot(A, A, i, j, m) + c1 * A[i][j] + (i == j ? c0 : 0.0);      // q
+        double vq[PER], va[PER];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int e = tid + 256 * q, i = e / M, j = e % M;
+            if (e < M * M) l.U[i][j] = c2 * ns_dot<M>(l.A, l.A, i, j) + c1 * l.A[i][j] + (i == j ? c0 : 0.0);      // q
         }
         __syncthreads();
-        for (int e = tid; e < m * m; e += 256) V[e / m][e % m] = ns_dot(U, Q, e / m, e % m, m);
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int e = tid + 256 * q, i = e / M, j = e % M;
+            if (e < M * M) {
+                vq[q] = ns_dot<M>(l.U, l.Q, i, j);
+                va[q] = ns_dot<M>(l.U, l.A, i, j);
+            }
+        }
         __syncthreads();
-        for (int e = tid; e < m * m; e += 256) Q[e / m][e % m] = V[e / m][e % m];
-        if (s + 1 == co.steps) break;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int e = tid + 256 * q, i = e / M, j = e % M;
+            if (e < M * M) {
+                l.Q[i][j] = vq[q];
+                l.V[i][j] = va[q];
+            }
+        }
         __syncthreads();
-        for (int e = tid; e < m * m; e += 256) V[e / m][e % m] = ns_dot(U, A, e / m, e % m, m);
-        __syncthreads();
-        for (int e = tid; e < m * m; e += 256) A[e / m][e % m] = ns_dot(V, U, e / m, e % m, m);
-        __syncthreads();
+        if (s + 1 < co.steps) {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                const int e = tid + 256 * q, i = e / M, j = e % M;
+                if (e < M * M) l.A[i][j] = ns_dot<M>(l.V, l.U, i, j);
+            }
+            __syncthreads();
+        }
     }
     fetch(0, false);
-    for (int j0 = 0; j0 < n; j0 += 64) {
+    for (int j0 = 0; j0 < n; j0 += JC) {
         __syncthreads();
         place();
         __syncthreads();
-        if (j0 + 64 < n) fetch(j0 + 64, false);
-        for (int e = tid; e < tasks; e += 256) {
-            const int i = e >> 6, j = e & 63;
-            if (j0 + j < n) {
+        if (j0 + JC < n) fetch(j0 + JC, false);
+#pragma unroll 2
+        for (int q = 0; q < 8; ++q) {
+            int i, j;
+            place_of(tid + 256 * q, i, j);
+            if (i < m && j0 + j < n) {
                 double s = 0.0;
-                for (int k = 0; k < m; ++k) s = fma(Q[i][k], (double)x[k][j], s);
+#pragma unroll 8
+                for (int k = 0; k < M; ++k) s = fma(l.Q[i][k], (double)l.x[k * LDX + j], s);
                 ns_update_out(a, d, b, i, j0 + j, (float)s);
             }
         }
     }
 }
 
+__global__ void __launch_bounds__(256) ns_norm_kernel(const NsTab a)
+{
+    __shared__ double red[4];
+    ns_norm(a, blockIdx.x, red);
+}
+
+// ---- the first launch of a chunk: whole small matrices, and the sums of squares of the others
+__global__ void __launch_bounds__(256) ns_first_kernel(const NsTab a, const NsCoef co, const int nsmall_wg)
+{
+    __shared__ NsSmallLds l;
+    const int id = blockIdx.x;
+    if (id < nsmall_wg) {
+        const int k = ns_find(a.small, a.nsmall, id), mi = a.nbig + k, b = id - a.small[k], m = a.mat[mi].m;
+        if (m <= 4) ns_small<4>(a, co, mi, b, l);
+        else if (m <= 8) ns_small<8>(a, co, mi, b, l);
+        else if (m <= 16) ns_small<16>(a, co, mi, b, l);
+        else ns_small<32>(a, co, mi, b, l);
+        return;
+    }
+    ns_norm(a, id - nsmall_wg, &l.A[0][0]);
+}
+
 inline int ns_pad(int v, int to) { return (v + to - 1) / to * to; }
 inline bool ns_is_small(const p2c_ns_matrix &m) { return (m.rows < m.cols ? m.rows : m.cols) <= NS_SMALL; }
 
 // Tile of a chunk's products: 128 keeps the matrix units busy (a wave reads 16 KB of operands for 24 instructions), 64 has four times the
-// workgroups and a shorter chain per workgroup.
+// workgroups and a shorter chain per workgroup.  The choice is made for the widest product (all tiles); the padding of the sides follows it.
 inline int ns_tile(const p2c_ns_matrix *mats, int n)
 {
     long long t128 = 0;
     for (int i = 0; i < n; ++i)
-        if (!ns_is_small(mats[i])) {
-            const int s = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols;
-            const long long mt = (s + 127) / 128;
-            t128 += mt * (mt + 1) / 2 * mats[i].batch;
-        }
+        if (!ns_is_small(mats[i])) t128 += (long long)((mats[i].rows + 127) / 128) * ((mats[i].cols + 127) / 128) * mats[i].batch;
     return t128 >= 256 ? 128 : 64;
 }
 
 inline size_t ns_one_ws(const p2c_ns_matrix &m, int tile)
 {
-    if (ns_is_small(m)) return 0;
+    if (ns_is_small(m) || !m.rows || !m.cols) return 0;
     const int s = m.rows < m.cols ? m.rows : m.cols, l = m.rows < m.cols ? m.cols : m.rows, mP = ns_pad(s, tile), nP = ns_pad(l, tile);
-    return NS_SLABS * 8 + 3 * ns_xbytes(mP, nP) + 2 * ns_xbytes(mP, mP);
+    return NS_PARTS * 8 + 3 * ns_xbytes(mP, nP) + 2 * ns_xbytes(mP, mP);
 }
 
 int ns_check(const p2c_ns_matrix *mats, int n)
@@ -459,83 +657,118 @@ int ns_check(const p2c_ns_matrix *mats, int n)
     return P2C_OK;
 }
 
-inline size_t ns_chunk_ws(const p2c_ns_matrix *mats, int n)
+template <int TB, int KG, int NST, int PH>
+int ns_product(const NsTab *tab, const NsRec *recs, int grid, float ca, float cb, int cur, hipStream_t st)
 {
-    const int tile = ns_tile(mats, n);
-    size_t s = 0;
-    for (int i = 0; i < n; ++i) s += ns_one_ws(mats[i], tile) * mats[i].batch;
-    return s;
+    constexpr int WG = TB == 32 ? 1 : 4, OUT = KG == 1 ? 4 * 32 * 36 * 4 : KG * WG * 4 * 64 * 16 + WG * 32 * 36 * 4, OPS = KG * 2 * TB * 128 * NST, LDS = OPS > OUT ? OPS : OUT;
+    static_assert(LDS <= 160 * 1024, "");
+    if (LDS > 65536) {
+        const hipError_t rc = hipFuncSetAttribute((const void *)ns_product_kernel<TB, KG, NST, PH>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (rc != hipSuccess) return (int)rc;
+    }
+    hipLaunchKernelGGL((ns_product_kernel<TB, KG, NST, PH>), dim3(grid), dim3((TB == 32 ? 64 : 256) * KG), LDS, st, tab, recs, ca, cb, cur);
+    P2C_LAUNCH_CHECK();
+    return P2C_OK;
 }
 
-template <int TB, int NST>
-int ns_products(NsArgs &a, const NsCoef &co, int total_sym, int total_all, const int *sym, const int *all, hipStream_t st)
+// The tile of one product of the chunk.  Few tiles: 32 with the k range shared by four waves - such a product is bound by the time its operands take
+// to arrive, and this form has the most of them in flight over the most CUs (products of the 19 backbone matrices, 405 tiles of 32: 10.2 and 7.6 us
+// against 14.0 and 9.0 with 64).  Many: it reads every operand twice as often (the decoder's seven 512 x 512, 988 tiles of 32: 20 us against 10).
+inline int ns_pick(const NsTab &a, bool sym, int pad)
 {
-    constexpr int LDS = 2 * TB * 128 * NST;
-    static_assert(LDS >= 4 * 32 * 36 * 4, "");
-    for (int s = 0; s < co.steps; ++s) {
-        const bool last = s + 1 == co.steps;
-        for (int i = 0; i <= a.nmat; ++i) a.start[i] = sym[i];
-        hipLaunchKernelGGL((ns_product_kernel<TB, NST, 1>), dim3(total_sym), dim3(256), LDS, st, a, 0.f, 1.f, s & 1);
-        P2C_LAUNCH_CHECK();
-        hipLaunchKernelGGL((ns_product_kernel<TB, NST, 2>), dim3(total_sym), dim3(256), LDS, st, a, co.c[s][1], co.c[s][2], s & 1);
-        P2C_LAUNCH_CHECK();
-        for (int i = 0; i <= a.nmat; ++i) a.start[i] = all[i];
-        if (last) hipLaunchKernelGGL((ns_product_kernel<TB, NST, 4>), dim3(total_all), dim3(256), LDS, st, a, co.c[s][0], 1.f, s & 1);
-        else hipLaunchKernelGGL((ns_product_kernel<TB, NST, 3>), dim3(total_all), dim3(256), LDS, st, a, co.c[s][0], 1.f, s & 1);
-        P2C_LAUNCH_CHECK();
+    long long t32 = 0;
+    for (int i = 0; i < a.nbig; ++i) {
+        const long long mt = a.mat[i].mP / 32, nt = a.mat[i].nP / 32;
+        t32 += (sym ? mt * (mt + 1) / 2 : mt * nt) * a.mat[i].batch;
     }
-    return P2C_OK;
+    return pad == 128 ? 128 : t32 <= 512 ? 32 : 64;
+}
+
+inline int ns_starts(NsTab &a, int phase, int tile)
+{
+    for (int i = 0; i < a.nbig; ++i) {
+        const int mt = a.mat[i].mP / tile, nt = a.mat[i].nP / tile;
+        a.start[phase][i + 1] = a.start[phase][i] + (phase == NS_SYM ? mt * (mt + 1) / 2 : mt * nt) * a.mat[i].batch;
+    }
+    return a.start[phase][a.nbig];
+}
+
+template <int PH>
+int ns_product_any(const NsTab *tab, const NsRec *recs, int tile, int grid, float ca, float cb, int cur, hipStream_t st)
+{
+    if (tile == 128) return ns_product<128, 1, 2, PH>(tab, recs, grid, ca, cb, cur, st);
+    if (tile == 64) return ns_product<64, 1, 4, PH>(tab, recs, grid, ca, cb, cur, st);
+    return ns_product<32, 4, 4, PH>(tab, recs, grid, ca, cb, cur, st);
+}
+
+// the chunk's table (without ws); returns the bytes of workspace it needs
+size_t ns_table(const p2c_ns_matrix *mats, int n, NsTab &a)
+{
+    const int tile = ns_tile(mats, n);
+    a.nbig = a.nsmall = 0;
+    a.start[NS_NORM][0] = a.start[NS_TILES][0] = a.start[NS_SYM][0] = a.start[NS_ALL][0] = a.small[0] = 0;
+    size_t off = 0;
+    for (int small = 0; small < 2; ++small)
+        for (int i = 0; i < n; ++i) {
+            const p2c_ns_matrix &q = mats[i];
+            if (!q.rows || !q.cols || !q.batch || (int)ns_is_small(q) != small) continue;
+            NsMat &d = a.mat[a.nbig + a.nsmall];
+            d.src = (const char *)q.src; d.mom = q.mom; d.dst = (char *)q.dst;
+            d.src_rs = q.src_rs; d.src_cs = q.src_cs; d.src_bs = q.src_bs;
+            d.dst_rs = q.dst_rs; d.dst_cs = q.dst_cs; d.dst_bs = q.dst_bs;
+            d.tall = q.rows > q.cols;
+            d.m = d.tall ? q.cols : q.rows; d.n = d.tall ? q.rows : q.cols;
+            d.mP = ns_pad(d.m, tile); d.nP = ns_pad(d.n, tile);
+            d.batch = q.batch; d.scale = q.scale; d.decay = q.decay;
+            d.ws = off; d.ws_bs = ns_one_ws(q, tile);
+            off += d.ws_bs * q.batch;
+            if (small) {
+                a.small[a.nsmall + 1] = a.small[a.nsmall] + q.batch;
+                ++a.nsmall;
+            } else {
+                const int j = a.nbig++;
+                a.start[NS_NORM][j + 1] = a.start[NS_NORM][j] + ns_parts(d.m, d.n) * q.batch;
+                a.start[NS_TILES][j + 1] = a.start[NS_TILES][j] + (d.mP / 64) * (d.nP / 64) * q.batch;
+            }
+        }
+    if (!a.nbig) return 0;
+    a.tsym = ns_pick(a, true, tile); a.tall = ns_pick(a, false, tile);
+    a.nsym = ns_starts(a, NS_SYM, a.tsym); a.nall = ns_starts(a, NS_ALL, a.tall);
+    const size_t head = ns_head(a.nsym, a.nall);
+    for (int i = 0; i < a.nbig; ++i) a.mat[i].ws += head;
+    return off + head;
 }
 
 int ns_chunk(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, const NsCoef &co, double eps, char *ws, hipStream_t st)
 {
-    NsArgs a, sm;
-    a.ws = ws; a.dtype = dtype; a.mu = mu; a.muon = muon; a.eps = eps; a.nmat = 0;
-    sm = a;
-    const int tile = ns_tile(mats, n);
-    int slabs[NS_MAX + 1] = {0}, tiles[NS_MAX + 1] = {0}, sym[NS_MAX + 1] = {0}, all[NS_MAX + 1] = {0};
-    size_t off = 0;
-    sm.start[0] = 0;
-    for (int i = 0; i < n; ++i) {
-        const p2c_ns_matrix &q = mats[i];
-        if (!q.rows || !q.cols || !q.batch) continue;           // nothing to do
-        const bool small = ns_is_small(q);
-        NsArgs &t = small ? sm : a;
-        NsMat &d = t.mat[t.nmat];
-        d.src = (const char *)q.src; d.mom = q.mom; d.dst = (char *)q.dst;
-        d.src_rs = q.src_rs; d.src_cs = q.src_cs; d.src_bs = q.src_bs;
-        d.dst_rs = q.dst_rs; d.dst_cs = q.dst_cs; d.dst_bs = q.dst_bs;
-        d.tall = q.rows > q.cols;
-        d.m = d.tall ? q.cols : q.rows; d.n = d.tall ? q.rows : q.cols;
-        d.mP = ns_pad(d.m, tile); d.nP = ns_pad(d.n, tile);
-        d.batch = q.batch; d.scale = q.scale; d.decay = q.decay;
-        d.ws = off; d.ws_bs = ns_one_ws(q, tile);
-        off += d.ws_bs * q.batch;
-        const int k = t.nmat++;
-        if (small) {
-            sm.start[k + 1] = sm.start[k] + q.batch;
-        } else {
-            const long long sl = ((long long)d.m * d.n + 1023) / 1024;
-            const int mt = d.mP / tile;
-            slabs[k + 1] = slabs[k] + (int)(sl < NS_SLABS ? sl : NS_SLABS) * q.batch;
-            tiles[k + 1] = tiles[k] + (d.mP / 64) * (d.nP / 64) * q.batch;
-            sym[k + 1] = sym[k] + mt * (mt + 1) / 2 * q.batch;
-            all[k + 1] = all[k] + mt * (d.nP / tile) * q.batch;
-        }
-    }
-    if (sm.nmat) {
-        hipLaunchKernelGGL(ns_small_kernel, dim3(sm.start[sm.nmat]), dim3(256), 0, st, sm, co);
+    NsTab a;
+    memset(&a, 0, sizeof a);
+    a.ws = ws; a.dtype = dtype; a.mu = mu; a.muon = muon; a.eps = eps;
+    ns_table(mats, n, a);
+    if (!(a.nbig + a.nsmall)) return P2C_OK;
+    // small matrices: in one launch with the sums of squares if those are few (the registers of ns_small leave two workgroups a CU)
+    const int nsm = a.small[a.nsmall], nno = a.start[NS_NORM][a.nbig], apart = nno > 512 || !nsm;
+    if (nsm) {
+        hipLaunchKernelGGL(ns_first_kernel, dim3(nsm + (apart ? 0 : nno)), dim3(256), 0, st, a, co, nsm);
         P2C_LAUNCH_CHECK();
     }
-    if (!a.nmat) return P2C_OK;
-    for (int i = 0; i <= a.nmat; ++i) a.start[i] = slabs[i];
-    hipLaunchKernelGGL(ns_norm_kernel, dim3(slabs[a.nmat]), dim3(256), 0, st, a);
+    if (nno && apart) {
+        hipLaunchKernelGGL(ns_norm_kernel, dim3(nno), dim3(256), 0, st, a);
+        P2C_LAUNCH_CHECK();
+    }
+    if (!a.nbig) return P2C_OK;
+    hipLaunchKernelGGL(ns_begin_kernel, dim3(a.start[NS_TILES][a.nbig]), dim3(256), 0, st, a);
     P2C_LAUNCH_CHECK();
-    for (int i = 0; i <= a.nmat; ++i) a.start[i] = tiles[i];
-    hipLaunchKernelGGL(ns_begin_kernel, dim3(tiles[a.nmat]), dim3(256), 0, st, a, NS_SLABS);
-    P2C_LAUNCH_CHECK();
-    return tile == 128 ? ns_products<128, 2>(a, co, sym[a.nmat], all[a.nmat], sym, all, st)
-                       : ns_products<64, 4>(a, co, sym[a.nmat], all[a.nmat], sym, all, st);
+    const NsTab *tab = (const NsTab *)ws;
+    const NsRec *rsym = (const NsRec *)(ws + NS_TAB_BYTES), *rall = rsym + a.nsym;
+    for (int s = 0; s < co.steps; ++s) {
+        int rc = ns_product_any<1>(tab, rsym, a.tsym, a.nsym, 0.f, 1.f, s & 1, st);
+        if (rc == P2C_OK) rc = ns_product_any<2>(tab, rsym, a.tsym, a.nsym, co.c[s][1], co.c[s][2], s & 1, st);
+        if (rc == P2C_OK) rc = s + 1 < co.steps ? ns_product_any<3>(tab, rall, a.tall, a.nall, co.c[s][0], 1.f, s & 1, st)
+                                                : ns_product_any<4>(tab, rall, a.tall, a.nall, co.c[s][0], 1.f, s & 1, st);
+        if (rc != P2C_OK) return rc;
+    }
+    return P2C_OK;
 }
 
 int ns_run(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, int steps, const float *coeffs, double eps, void *ws, size_t ws_bytes,
@@ -552,8 +785,8 @@ int ns_run(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, int 
         const double c0 = coeffs[3 * s], c1 = coeffs[3 * s + 1], c2 = coeffs[3 * s + 2];
         if (!isfinite(c0) || !isfinite(c1) || !isfinite(c2)) return P2C_EINVAL;
         double p = 0.0, q = 0.0;
-        for (int k = 0; k <= 256; ++k) {
-            const double x = top * k / 256, t = x * x, bb = c1 * t + c2 * t * t, qq = c0 + bb;
+        for (int k = 0; k <= 64; ++k) {
+            const double x = top * k / 64, t = x * x, bb = c1 * t + c2 * t * t, qq = c0 + bb;
             p = fmax(p, fabs(x * qq));
             q = fmax(q, fmax(fabs(bb), fabs(c0)));
         }
@@ -567,8 +800,9 @@ int ns_run(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, int 
         if (q.rows && q.cols && q.batch && (!q.src || !q.dst || (muon && (!q.mom || q.batch != 1)))) return P2C_EINVAL;
     }
     size_t need = 0;
+    NsTab tab;
     for (int i = 0; i < n; i += NS_MAX) {
-        const size_t c = ns_chunk_ws(mats + i, n - i < NS_MAX ? n - i : NS_MAX);
+        const size_t c = ns_table(mats + i, n - i < NS_MAX ? n - i : NS_MAX, tab);
         need = c > need ? c : need;
     }
     if (need > ws_bytes || (need && (!ws || ((uintptr_t)ws & 15)))) return P2C_EINVAL;
@@ -585,8 +819,9 @@ extern "C" size_t p2c_newton_schulz_ws_bytes(const p2c_ns_matrix *mats_host, int
 {
     if (ns_check(mats_host, n) != P2C_OK) return 0;
     size_t need = 0;
+    NsTab tab;
     for (int i = 0; i < n; i += NS_MAX) {
-        const size_t c = ns_chunk_ws(mats_host + i, n - i < NS_MAX ? n - i : NS_MAX);
+        const size_t c = ns_table(mats_host + i, n - i < NS_MAX ? n - i : NS_MAX, tab);
         need = c > need ? c : need;
     }
     return need;

@@ -5,6 +5,7 @@ stream to libp2c_hip.so, and register backward passes with torch.autograd.  No a
 path happens in torch ops in this file.  All feature tensors are POINT-MAJOR: [rows, channels].
 """
 import ctypes
+import functools
 import os
 import struct
 
@@ -1554,7 +1555,12 @@ assert _NS_RECORD.size == ctypes.sizeof(_lib.NsMatrix)
 
 def ns_coefficients(steps, coeffs):
     """-> ctypes float [steps * 3]: one (a, b, c) for all steps, or one per step."""
-    steps = int(steps)
+    flat = tuple(coeffs) if not hasattr(coeffs[0], "__len__") else tuple(tuple(c) for c in coeffs)
+    return _ns_coefficients(int(steps), flat)
+
+
+@functools.lru_cache(maxsize=64)             # (0.2 ms of Python to check them)
+def _ns_coefficients(steps, coeffs):
     if not 1 <= steps <= 16:
         raise ValueError("newton_schulz: steps = %d is outside 1 ... 16" % steps)
     rows = [tuple(coeffs)] * steps if not hasattr(coeffs[0], "__len__") else [tuple(c) for c in coeffs]

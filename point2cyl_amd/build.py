@@ -27,7 +27,7 @@ FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=o
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # kernels that are short and launched in chains: their arguments arrive in registers (16 of them) instead of through a cold miss
-EXTRA = {"muon.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
+EXTRA = {f: ["-mllvm", "-amdgpu-kernarg-preload-count=16"] for f in ("muon.hip", "int8.hip")}
 
 
 def source_hash():

@@ -52,6 +52,7 @@ struct NsTab {
     int muon;                           // 0 orthogonalise, 1 momentum, 2 Nesterov momentum
     double eps;
     int nsym, nall, tsym, tall;         // products: workgroups and tile of the symmetric ones, of the others
+    int mid, unused;                    // every tiled matrix fits ns_mid_kernel
     int start[4][NS_MAX + 1];
     int small[NS_MAX + 1];
     NsMat mat[NS_MAX];
@@ -71,42 +72,68 @@ template <class D> __device__ __forceinline__ char *ns_T(char *w, const D &d, in
 template <class D> __device__ __forceinline__ char *ns_A(char *w, const D &d) { return ns_S(w) + 3 * ns_xbytes(d.mP, d.nP); }
 template <class D> __device__ __forceinline__ char *ns_B(char *w, const D &d) { return ns_A(w, d) + ns_xbytes(d.mP, d.mP); }
 
-__device__ __forceinline__ float ns_get(const char *p, long long i, int dt)
-{
-    if (dt == 0) return reinterpret_cast<const float *>(p)[i];
-    if (dt == 1) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << 16);
-    return (float)reinterpret_cast<const _Float16 *>(p)[i];
-}
-__device__ __forceinline__ void ns_put(char *p, long long i, int dt, float v)
-{
-    if (dt == 0) reinterpret_cast<float *>(p)[i] = v;
-    else if (dt == 1) reinterpret_cast<__bf16 *>(p)[i] = (__bf16)v;
-    else reinterpret_cast<_Float16 *>(p)[i] = (_Float16)v;
-}
-
-// u of row r, column c; first: the momentum is advanced, else the advanced one is read
-__device__ __forceinline__ float ns_update_in(const NsTab &a, const NsMat &d, const char *src, int r, int c, bool first)
-{
-    const float g = ns_get(src, r * d.src_rs + c * d.src_cs, a.dtype);
-    if (!a.muon) return g;
-    float *mp = d.mom + (long long)r * (d.tall ? d.m : d.n) + c;
-    float mv = *mp;
-    if (first) {
-        mv = __builtin_fmaf(a.mu, mv, (1.0f - a.mu) * g);
-        *mp = mv;
-    }
-    return a.muon == 2 ? __builtin_fmaf(a.mu, mv, (1.0f - a.mu) * g) : mv;
-}
 __device__ __forceinline__ const char *ns_src(const NsTab &a, const NsMat &d, int b) { return d.src + b * d.src_bs * (a.dtype == 0 ? 4 : 2); }
 
-// O's element (i of the small side, j of the long one): stored, or taken off the parameter
-__device__ __forceinline__ void ns_update_out(const NsTab &a, const NsMat &d, int b, int i, int j, float o)
+// What differs between calls (type, momentum) is decided once per group of N elements, so that their loads are in flight together: decided per element
+// they wait for each other (32 of them: 14000 clocks).
+// G of N elements: at(q) = offset in elements, always one of the matrix
+template <int N, class At>
+__device__ __forceinline__ void ns_load_n(const char *src, int dtype, float (&v)[N], At at)
 {
-    const long long r = d.tall ? j : i, c = d.tall ? i : j;
-    const long long at = b * d.dst_bs + r * d.dst_rs + c * d.dst_cs;
-    if (!a.muon) { ns_put(d.dst, at, a.dtype, o); return; }
-    float *p = reinterpret_cast<float *>(d.dst) + at;
-    *p = *p * d.decay - d.scale * o;
+    if (dtype == 0) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = reinterpret_cast<const float *>(src)[at(q)];
+    } else if (dtype == 1) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(src)[at(q)] << 16);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = (float)reinterpret_cast<const _Float16 *>(src)[at(q)];
+    }
+}
+// u of N elements from G and the momentum; first: the momentum is advanced, else the advanced one is read.  at_m(q): its offset; ok(q): the element exists
+template <int N, class At, class Ok>
+__device__ __forceinline__ void ns_momentum_n(const NsTab &a, float *mom, float (&v)[N], bool first, At at_m, Ok ok)
+{
+    float m[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) m[q] = mom[at_m(q)];
+    if (first) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) m[q] = __builtin_fmaf(a.mu, m[q], (1.0f - a.mu) * v[q]);
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (ok(q)) mom[at_m(q)] = m[q];
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = a.muon == 2 ? __builtin_fmaf(a.mu, m[q], (1.0f - a.mu) * v[q]) : m[q];
+}
+// N elements of the result: stored, or taken off the parameter.  i of the small side, j of the long one
+template <int N, class I, class J>
+__device__ __forceinline__ void ns_store_n(const NsTab &a, const NsMat &d, int b, const float (&o)[N], I i, J j)
+{
+    auto ok = [&](int q) { return i(q) < d.m && j(q) < d.n; };
+    auto at = [&](int q) { return b * d.dst_bs + (d.tall ? j(q) : i(q)) * d.dst_rs + (d.tall ? i(q) : j(q)) * d.dst_cs; };
+    if (a.muon) {
+        float *p = reinterpret_cast<float *>(d.dst), v[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = ok(q) ? p[at(q)] : 0.f;
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (ok(q)) p[at(q)] = v[q] * d.decay - d.scale * o[q];
+    } else if (a.dtype == 0) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (ok(q)) reinterpret_cast<float *>(d.dst)[at(q)] = o[q];
+    } else if (a.dtype == 1) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (ok(q)) reinterpret_cast<__bf16 *>(d.dst)[at(q)] = (__bf16)o[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (ok(q)) reinterpret_cast<_Float16 *>(d.dst)[at(q)] = (_Float16)o[q];
+    }
 }
 
 // workgroup -> matrix; everything uniform
@@ -135,12 +162,15 @@ __device__ __forceinline__ void ns_split8(const float *v, h16x8 &hi, h16x8 &lo)
     }
 }
 
-// 64 x 64 elements of a matrix in 16 registers a thread, 16 loads in flight: rows r0 + (tid >> 6) + 4 q, column c0 + (tid & 63)
+// 64 x 64 elements of a matrix in 16 registers a thread, 16 loads in flight: rows r0 + (tid >> 6) + 4 q, column c0 + (tid & 63); zeros outside
 __device__ __forceinline__ void ns_load_tile(const NsTab &a, const NsMat &d, const char *src, int r0, int c0, bool first, float (&v)[16])
 {
-    const int rows = d.tall ? d.n : d.m, cols = d.tall ? d.m : d.n, r = r0 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63);
+    const int rows = d.tall ? d.n : d.m, cols = d.tall ? d.m : d.n, r = r0 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63), cc = min(c, cols - 1);
+    auto ok = [&](int q) { return r + 4 * q < rows && c < cols; };
+    ns_load_n(src, a.dtype, v, [&](int q) { return min(r + 4 * q, rows - 1) * d.src_rs + cc * d.src_cs; });
+    if (a.muon) ns_momentum_n(a, d.mom, v, first, [&](int q) { return (long long)min(r + 4 * q, rows - 1) * cols + cc; }, ok);
 #pragma unroll
-    for (int q = 0; q < 16; ++q) v[q] = (r + 4 * q < rows && c < cols) ? ns_update_in(a, d, src, r + 4 * q, c, first) : 0.f;
+    for (int q = 0; q < 16; ++q) v[q] = ok(q) ? v[q] : 0.f;
 }
 
 // partial sums of a matrix: one per 64 x 64 tile of it, at most NS_PARTS
@@ -367,10 +397,13 @@ __global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(
     auto last = [&](const float *stage, int x, int y, int first, int count) {
         const NsMat &m = tab->mat[d.mi];
         const int i0 = tj * TB + wc + y * 32, j0 = ti * TB + wr + x * 32;
-#pragma unroll 4
-        for (int e = first; e < 1024; e += count) {
-            const int u = e >> 5, v = e & 31, i = m.tall ? v : u, j = m.tall ? u : v;
-            if (i0 + i < m.m && j0 + j < m.n) ns_update_out(*tab, m, d.b, i0 + i, j0 + j, stage[j * LDS_ + i] * NS_INV);
+        for (int e0 = first; e0 < 1024; e0 += 4 * count) {
+            float o[4];
+            auto i = [&](int q) { const int e = e0 + q * count; return m.tall ? e & 31 : e >> 5; };
+            auto j = [&](int q) { const int e = e0 + q * count; return m.tall ? e >> 5 : e & 31; };
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o[q] = stage[j(q) * LDS_ + i(q)] * NS_INV;
+            ns_store_n(*tab, m, d.b, o, [&](int q) { return i0 + i(q); }, [&](int q) { return j0 + j(q); });
         }
     };
     if (KG == 1) {
@@ -449,11 +482,387 @@ __global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(
     }
 }
 
+struct NsCoef { int steps; float c[16][3]; };
+
+// 8 elements from offset `at` on, `cs` apart, of which `left` exist (zeros for the others): in 16-byte pieces where they are whole and neighbours
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef u16x8 u16x8_u __attribute__((aligned(2)));
+__device__ __forceinline__ float ns_wide(uint16_t u, int dtype) { return dtype == 1 ? __uint_as_float((uint32_t)u << 16) : (float)__builtin_bit_cast(_Float16, u); }
+__device__ __forceinline__ uint16_t ns_narrow(float v, int dtype) { return dtype == 1 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v); }
+__device__ __forceinline__ void ns_get8(const char *p, long long at, long long cs, int left, int dtype, float (&v)[8])
+{
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    if (left >= 8 && cs == 1) {
+        if (dtype == 0) {
+            const f32x4_u *q = reinterpret_cast<const f32x4_u *>(p + at * 4);
+            const f32x4 x = q[0], y = q[1];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[k] = x[k]; v[4 + k] = y[k]; }
+        } else {
+            const u16x8 x = *reinterpret_cast<const u16x8_u *>(p + at * 2);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = ns_wide(x[k], dtype);
+        }
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k)
+            if (k < left) {
+                const float x = dtype == 0 ? *reinterpret_cast<const float *>(p + (at + k * cs) * 4) : ns_wide(*reinterpret_cast<const uint16_t *>(p + (at + k * cs) * 2), dtype);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e == k ? x : v[e];
+            }
+    }
+}
+__device__ __forceinline__ void ns_put8(char *p, long long at, long long cs, int left, int dtype, const float (&v)[8])
+{
+    if (left >= 8 && cs == 1) {
+        if (dtype == 0) {
+            f32x4_u *q = reinterpret_cast<f32x4_u *>(p + at * 4);
+            q[0] = f32x4{v[0], v[1], v[2], v[3]};
+            q[1] = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            u16x8 x;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = ns_narrow(v[k], dtype);
+            *reinterpret_cast<u16x8_u *>(p + at * 2) = x;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) {
+                if (dtype == 0) *reinterpret_cast<float *>(p + (at + k * cs) * 4) = v[k];
+                else *reinterpret_cast<uint16_t *>(p + (at + k * cs) * 2) = ns_narrow(v[k], dtype);
+            }
+    }
+}
+
+// ---- matrices of up to 16384 elements (sides padded to 64: 128 x 128, 64 x 256): one workgroup each, all steps without leaving LDS.  The tiled form is
+// a chain of 17 launches of 4 us; here a step is three products of 1.5 us (both operands of a 128 x 128 product out of LDS: 384 KB, as long as its
+// matrix instructions).  S, then A, then B share one region: S is read by the first product only, and a X comes from the registers, which hold X in 32
+// bits in the layout of the products' results.  Measured at 128 x 128: 64 -> 50 us a call.
+constexpr int NS_MID = 16384;
+
+struct NsMidImage { int base, rows; };                          // offset in LDS; [k-tile][row][128 bytes], chunks permuted as in tile_dma.h
+
+// offset of the hi chunk of 8 k; the lo chunk is 16 bytes apart before the permutation (chunk c and c ^ 1): its offset is this one ^ 16
+__device__ __forceinline__ int ns_mid_at(const NsMidImage &m, int row, int k) { return m.base + (k >> 5) * (m.rows * 128) + p2c_tile_at<128>(row, (k & 31) >> 3 << 1); }
+
+// 16 values of a lane (rows 8 g + 4 h + 0..3 of a 32 x 32 piece, times a power of two) as 4 x 4 consecutive k of image row `row`, k-tile k0 / 32
+__device__ __forceinline__ void ns_mid_split4(const f32x16 &v, int g, float f, h16x4 &hi, h16x4 &lo)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = (_Float16)(v[4 * g + e] * f);
+        lo[e] = (_Float16)__builtin_fmaf(v[4 * g + e], f, -(float)hi[e]);
+    }
+}
+__device__ __forceinline__ void ns_mid_put(char *lds, const NsMidImage &m, int row, int k0, int h, const f32x16 &v, float f)
+{
+    const int at = ns_mid_at(m, row, k0) + 8 * h;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        h16x4 hi, lo;
+        ns_mid_split4(v, g, f, hi, lo);
+        *reinterpret_cast<h16x4 *>(lds + (at ^ (32 * g))) = hi;
+        *reinterpret_cast<h16x4 *>(lds + (at ^ (32 * g + 16))) = lo;
+    }
+}
+
+// 4 x 4 half words across a quad of lanes: in, word e of lane q is M[e][q]; out, lane q holds M[q][0..3]
+__device__ __forceinline__ uint2 ns_quad_transpose(uint2 r, int lane)
+{
+    const uint32_t sel = lane & 1 ? 0x03020706u : 0x05040100u;             // odd: {high of the partner, own high}; even: {own low, low of the partner}
+    const uint32_t a0 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.x), r.x, sel), a1 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.y), r.y, sel);
+    const bool up = (lane & 2) != 0;
+    const uint32_t y = (uint32_t)p2c_dpp<0x4E>((int)(up ? a0 : a1));
+    return up ? make_uint2(y, a1) : make_uint2(a0, y);
+}
+
+__global__ void __launch_bounds__(512) ns_mid_kernel(const NsTab a, const NsCoef co)
+{
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int mi = ns_find(a.start[NS_ALL], a.nbig, blockIdx.x);
+    const NsMat &d = a.mat[mi];
+    const int b = blockIdx.x - a.start[NS_ALL][mi], tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), il = lane & 31, h = lane >> 5;
+    const int mt = d.mP >> 5, nt = d.nP >> 5, xb = d.mP * d.nP * 4;
+    const NsMidImage S = {0, d.mP}, T = {xb, d.nP};               // A and B are images of mP rows in S's place
+    double *red = reinterpret_cast<double *>(smem + 2 * xb);
+
+    // ---- the matrix: 8 consecutive columns of a row per unit, at most 4 units a thread
+    const int rows = d.tall ? d.n : d.m, cols = d.tall ? d.m : d.n, c8n = (d.tall ? d.mP : d.nP) >> 3, units = (d.tall ? d.nP : d.mP) * c8n;
+    const char *src = ns_src(a, d, b);
+    const float rc8 = 1.0f / c8n;
+    int ur[4], uc[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int u = tid + 512 * q;
+        ur[q] = (int)((u + 0.5f) * rc8);                        // u / c8n (u < 2048)
+        uc[q] = (u - ur[q] * c8n) * 8;
+    }
+    float v[4][8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int left = tid + 512 * q < units && ur[q] < rows ? cols - uc[q] : 0;
+        ns_get8(src, ur[q] * d.src_rs + uc[q] * d.src_cs, d.src_cs, left, a.dtype, v[q]);
+    }
+    if (a.muon) {
+        float m[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int left = tid + 512 * q < units && ur[q] < rows ? cols - uc[q] : 0;
+            ns_get8((const char *)d.mom, (long long)ur[q] * cols + uc[q], 1, left, 0, m[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int left = tid + 512 * q < units && ur[q] < rows ? cols - uc[q] : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                m[q][k] = __builtin_fmaf(a.mu, m[q][k], (1.0f - a.mu) * v[q][k]);
+                v[q][k] = a.muon == 2 ? __builtin_fmaf(a.mu, m[q][k], (1.0f - a.mu) * v[q][k]) : m[q][k];
+            }
+            ns_put8((char *)d.mom, (long long)ur[q] * cols + uc[q], 1, left, 0, m[q]);
+        }
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = fma((double)v[q][k], (double)v[q][k], s);
+    s = p2c_wave_sum_f64(s);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += red[k];
+    const double inv = (double)NS_SCALE / (sqrt(s) + a.eps);
+    const float finv = (float)inv;
+    if (finv > 1e-30f && finv < 1e30f) {                        // the factor of ordinary magnitudes is a 32-bit number
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[q][k] *= finv;
+    } else {
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {                           // (in two factors, each in range)
+            const double half = e ? inv / (double)(float)sqrt(inv) : (double)(float)sqrt(inv);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[q][k] = (float)((double)v[q][k] * half);
+        }
+    }
+    const NsMidImage &R = d.tall ? T : S, &C = d.tall ? S : T;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (tid + 512 * q < units) {
+            float w[8];
+            h16x8 hi, lo;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = v[q][k];
+            ns_split8(w, hi, lo);
+            const int at = ns_mid_at(R, ur[q], uc[q]);
+            *reinterpret_cast<h16x8 *>(smem + at) = hi;
+            *reinterpret_cast<h16x8 *>(smem + (at ^ 16)) = lo;
+        }
+    __syncthreads();
+
+    // fragments: row block `rb` of an image at k-step ks (16 k), plane pl
+    auto frag = [&](const NsMidImage &m, int rb, int ks, int pl) {
+        return *reinterpret_cast<const h16x8 *>(smem + (ns_mid_at(m, rb * 32 + il, ks * 16 + 8 * h) ^ (16 * pl)));
+    };
+    h16x8 one[2];                                               // the unit matrix of one k-tile as a fragment: a product with it re-lays a matrix exactly
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) one[t][e] = (_Float16)(16 * t + 8 * h + e == il ? 1.f : 0.f);
+    auto clear = [&](f32x16 &c) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) c[r] = 0.f;
+    };
+    // C[row block rb][column block cb] of an image itself: lane = column, rows in the registers
+    auto self = [&](const NsMidImage &m, int rb, int cb, f32x16 &c) {
+        clear(c);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int pl = 1; pl >= 0; --pl) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag(m, rb, 2 * cb + t, pl), one[t], c, 0, 0, 0);
+    };
+    f32x16 acc[2], x[2];
+    // the other image
+    const int rbn = R.rows >> 5, pairs = C.rows >> 6;           // at most 8 units of 32 rows x 64 columns: one a wave, here and in every product
+    if (wave < rbn * pairs) {
+        const int rb = wave / pairs, cb = wave % pairs * 2;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            self(R, rb, cb + y, acc[y]);
+            ns_mid_put(smem, C, (cb + y) * 32 + il, rb * 32, h, acc[y], 1.0f);
+        }
+    }
+    const int mp = mt >> 1, r3 = wave / mp, c3 = wave % mp * 2;  // this wave's unit: of the m x m products where it is one, of T'
+    const bool in_sym = wave < mt * mp, in_all = wave < nt * mp;
+    if (in_all) {                                               // X in the layout of T': lane = i, j in the registers; from the image that is there
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            if (d.tall) {
+                self(T, r3, c3 + y, x[y]);
+            } else {
+                clear(x[y]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int pl = 1; pl >= 0; --pl) x[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(one[t], frag(S, c3 + y, 2 * r3 + t, pl), x[y], 0, 0, 0);
+            }
+        }
+    }
+    __syncthreads();
+    // A k-tile's fragments (chunk 2 (2 s + h) + pl of a row: s and pl are bits 6 and 4 of its offset, whatever the permutation) are read while the one
+    // before is multiplied: read and multiplied in turn, a product took 6100 clocks for 3100 of either.
+    struct Frags { h16x8 p[2][2], q[2][2][2]; };
+    auto product = [&](const NsMidImage &p, const NsMidImage &q, int KT) {
+        clear(acc[0]);
+        clear(acc[1]);
+        int op = ns_mid_at(p, r3 * 32 + il, 8 * h), oq[2] = {ns_mid_at(q, c3 * 32 + il, 8 * h), ns_mid_at(q, c3 * 32 + 32 + il, 8 * h)};
+        const int sp = p.rows * 128, sq = q.rows * 128;
+        auto read = [&](Frags &f) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) {
+                    f.p[t][pl] = *reinterpret_cast<const h16x8 *>(smem + (op ^ (64 * t + 16 * pl)));
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) f.q[t][y][pl] = *reinterpret_cast<const h16x8 *>(smem + (oq[y] ^ (64 * t + 16 * pl)));
+                }
+            op += sp;
+            oq[0] += sq;
+            oq[1] += sq;
+        };
+        auto multiply = [&](const Frags &f) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[t][pr == 1], f.q[t][y][pr == 0], acc[y], 0, 0, 0);
+        };
+        Frags f0, f1;
+        read(f0);
+        for (int kt = 0; kt < KT; kt += 2) {                    // (KT is even: the sides are multiples of 64)
+            read(f1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kt + 2 < KT) read(f0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (int st = 0; st < co.steps; ++st) {
+        const float c0 = co.c[st][0], c1 = co.c[st][1], c2 = co.c[st][2];
+        asm volatile("" ::"s"(c0), "s"(c1), "s"(c2));           // here now: a scalar load in flight would make every wait below a wait for all of LDS
+        if (in_sym) product(S, S, nt);
+        __syncthreads();
+        if (in_sym) {                                           // (A is symmetric: its transposed image is its image)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) ns_mid_put(smem, S, (c3 + y) * 32 + il, r3 * 32, h, acc[y], NS_INV);
+        }
+        __syncthreads();
+        if (in_sym) {
+            product(S, S, mt);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int at = ns_mid_at(S, (c3 + y) * 32 + il, r3 * 32) + 8 * h;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const h16x4 oh = *reinterpret_cast<const h16x4 *>(smem + (at ^ (32 * g))), ol = *reinterpret_cast<const h16x4 *>(smem + (at ^ (32 * g + 16)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[y][4 * g + e] = __builtin_fmaf(c1, (float)oh[e] + (float)ol[e], (c2 * NS_INV) * acc[y][4 * g + e]);
+                }
+            }
+        }
+        __syncthreads();
+        if (in_sym) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) ns_mid_put(smem, S, (c3 + y) * 32 + il, r3 * 32, h, acc[y], 1.0f);
+        }
+        __syncthreads();
+        if (in_all) {
+            product(T, S, mt);
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[y][r] = __builtin_fmaf(c0, x[y][r], acc[y][r] * NS_INV);
+        }
+        if (st + 1 == co.steps) break;
+        __syncthreads();
+        if (in_all) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int i = (c3 + y) * 32 + il, at = ns_mid_at(S, i, r3 * 32) + 8 * h;
+                // T': rows r3 32 + 8 g + 4 h + (lane & 3), columns of the lane's quad; 8 rows on, the permutation's bits 4-6 change by (8 / 2) << 4
+                const int i4 = i & ~3, at_t = ns_mid_at(T, r3 * 32 + 4 * h + (lane & 3), i4) + (i4 & 4) * 2;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    h16x4 hi, lo;
+                    ns_mid_split4(x[y], g, 1.0f, hi, lo);
+                    *reinterpret_cast<h16x4 *>(smem + (at ^ (32 * g))) = hi;
+                    *reinterpret_cast<h16x4 *>(smem + (at ^ (32 * g + 16))) = lo;
+                    const uint2 th = ns_quad_transpose(__builtin_bit_cast(uint2, hi), lane), tl = ns_quad_transpose(__builtin_bit_cast(uint2, lo), lane);
+                    const int t = (at_t + g * 1024) ^ ((g & 1) * 64);
+                    *reinterpret_cast<uint2 *>(smem + t) = th;
+                    *reinterpret_cast<uint2 *>(smem + (t ^ 16)) = tl;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // the result through LDS (the images are done with), out 8 columns of a row at a time
+    __syncthreads();
+    float *stage = reinterpret_cast<float *>(smem);
+    const int lds = (d.tall ? d.mP : d.nP) + 4;                 // (16384 + 4 x 256 floats at most: within the two images)
+    if (in_all) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int i = (c3 + y) * 32 + il, j = r3 * 32 + 8 * g + 4 * h;
+                if (d.tall) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) stage[(j + e) * lds + i] = x[y][4 * g + e];
+                } else {
+                    *reinterpret_cast<f32x4 *>(stage + i * lds + j) = f32x4{x[y][4 * g], x[y][4 * g + 1], x[y][4 * g + 2], x[y][4 * g + 3]};
+                }
+            }
+    }
+    __syncthreads();
+    char *dst = d.dst + b * d.dst_bs * (a.dtype == 0 ? 4 : 2);
+    float o[4][8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int left = tid + 512 * q < units && ur[q] < rows ? cols - uc[q] : 0;
+        if (a.muon) ns_get8(dst, ur[q] * d.dst_rs + uc[q] * d.dst_cs, d.dst_cs, left, 0, o[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int left = tid + 512 * q < units && ur[q] < rows ? cols - uc[q] : 0;
+        if (left > 0) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(stage + ur[q] * lds + uc[q]), hi = *reinterpret_cast<const f32x4 *>(stage + ur[q] * lds + uc[q] + 4);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float r = (k < 4 ? lo[k & 3] : hi[k & 3]) * NS_INV;
+                o[q][k] = a.muon ? o[q][k] * d.decay - d.scale * r : r;
+            }
+            ns_put8(dst, ur[q] * d.dst_rs + uc[q] * d.dst_cs, d.dst_cs, left, a.dtype, o[q]);
+        }
+    }
+}
+
 // ---- small side <= 32: one workgroup per matrix, in the m x m space and in 64 bits.  X_k = Q_k X_0 with Q and A polynomials of A_0 = X_0 X_0^T:
 // q = a + bA + cA^2, Q <- q Q, A <- q A q.  G is read twice and nothing else moves.  64 bits are what this form needs (A holds SQUARED singular
 // values and a rounding grows by a^2 per step: 2.5e5 over five); at this size they cost less than the launches of the tiled form.
-struct NsCoef { int steps; float c[16][3]; };
-
 constexpr int NS_XS = 2112;                                     // floats of a chunk of X: m rows of 64 ... 2048 elements, each padded by one
 
 struct NsSmallLds {
@@ -487,13 +896,15 @@ __device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int m
         if (d.tall) { i = e % M; j = e / M; } else { i = e / JC; j = e % JC; }
     };
     auto fetch = [&](int j0, bool first) {
+        auto ii = [&](int q) { int i, j; place_of(tid + 256 * q, i, j); return i; };
+        auto jj = [&](int q) { int i, j; place_of(tid + 256 * q, i, j); return j0 + j; };
+        auto ok = [&](int q) { return ii(q) < m && jj(q) < n; };
+        auto row = [&](int q) { return d.tall ? min(jj(q), n - 1) : min(ii(q), m - 1); };
+        auto col = [&](int q) { return d.tall ? min(ii(q), m - 1) : min(jj(q), n - 1); };
+        ns_load_n(src, a.dtype, nx, [&](int q) { return row(q) * d.src_rs + col(q) * d.src_cs; });
+        if (a.muon) ns_momentum_n(a, d.mom, nx, first, [&](int q) { return (long long)row(q) * (d.tall ? m : n) + col(q); }, ok);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            int i, j;
-            place_of(tid + 256 * q, i, j);
-            j += j0;
-            nx[q] = (i < m && j < n) ? ns_update_in(a, d, src, d.tall ? j : i, d.tall ? i : j, first) : 0.f;
-        }
+        for (int q = 0; q < 8; ++q) nx[q] = ok(q) ? nx[q] : 0.f;
     };
     auto place = [&]() {
 #pragma unroll
@@ -592,17 +1003,17 @@ __device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int m
         place();
         __syncthreads();
         if (j0 + JC < n) fetch(j0 + JC, false);
+        float o[8];
 #pragma unroll 2
         for (int q = 0; q < 8; ++q) {
             int i, j;
             place_of(tid + 256 * q, i, j);
-            if (i < m && j0 + j < n) {
-                double s = 0.0;
+            double s = 0.0;
 #pragma unroll 8
-                for (int k = 0; k < M; ++k) s = fma(l.Q[i][k], (double)l.x[k * LDX + j], s);
-                ns_update_out(a, d, b, i, j0 + j, (float)s);
-            }
+            for (int k = 0; k < M; ++k) s = fma(l.Q[i][k], (double)l.x[k * LDX + j], s);
+            o[q] = (float)s;
         }
+        ns_store_n(a, d, b, o, [&](int q) { int i, j; place_of(tid + 256 * q, i, j); return i; }, [&](int q) { int i, j; place_of(tid + 256 * q, i, j); return j0 + j; });
     }
 }
 
@@ -639,6 +1050,14 @@ inline int ns_tile(const p2c_ns_matrix *mats, int n)
     for (int i = 0; i < n; ++i)
         if (!ns_is_small(mats[i])) t128 += (long long)((mats[i].rows + 127) / 128) * ((mats[i].cols + 127) / 128) * mats[i].batch;
     return t128 >= 256 ? 128 : 64;
+}
+
+// every matrix of the chunk that is not small fits one workgroup (together with larger ones they ride in the tiled products at no cost)
+inline bool ns_all_mid(const p2c_ns_matrix *mats, int n)
+{
+    for (int i = 0; i < n; ++i)
+        if (!ns_is_small(mats[i]) && (long long)ns_pad(mats[i].rows, 64) * ns_pad(mats[i].cols, 64) > NS_MID) return false;
+    return true;
 }
 
 inline size_t ns_one_ws(const p2c_ns_matrix &m, int tile)
@@ -704,7 +1123,8 @@ int ns_product_any(const NsTab *tab, const NsRec *recs, int tile, int grid, floa
 // the chunk's table (without ws); returns the bytes of workspace it needs
 size_t ns_table(const p2c_ns_matrix *mats, int n, NsTab &a)
 {
-    const int tile = ns_tile(mats, n);
+    const bool mid = ns_all_mid(mats, n);
+    const int tile = mid ? 64 : ns_tile(mats, n);
     a.nbig = a.nsmall = 0;
     a.start[NS_NORM][0] = a.start[NS_TILES][0] = a.start[NS_SYM][0] = a.start[NS_ALL][0] = a.small[0] = 0;
     size_t off = 0;
@@ -727,11 +1147,13 @@ size_t ns_table(const p2c_ns_matrix *mats, int n, NsTab &a)
                 ++a.nsmall;
             } else {
                 const int j = a.nbig++;
+                if (mid) a.start[NS_ALL][j + 1] = a.start[NS_ALL][j] + q.batch;
                 a.start[NS_NORM][j + 1] = a.start[NS_NORM][j] + ns_parts(d.m, d.n) * q.batch;
                 a.start[NS_TILES][j + 1] = a.start[NS_TILES][j] + (d.mP / 64) * (d.nP / 64) * q.batch;
             }
         }
-    if (!a.nbig) return 0;
+    a.mid = mid;
+    if (!a.nbig || mid) return 0;
     a.tsym = ns_pick(a, true, tile); a.tall = ns_pick(a, false, tile);
     a.nsym = ns_starts(a, NS_SYM, a.tsym); a.nall = ns_starts(a, NS_ALL, a.tall);
     const size_t head = ns_head(a.nsym, a.nall);
@@ -747,7 +1169,7 @@ int ns_chunk(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, co
     ns_table(mats, n, a);
     if (!(a.nbig + a.nsmall)) return P2C_OK;
     // small matrices: in one launch with the sums of squares if those are few (the registers of ns_small leave two workgroups a CU)
-    const int nsm = a.small[a.nsmall], nno = a.start[NS_NORM][a.nbig], apart = nno > 512 || !nsm;
+    const int nsm = a.small[a.nsmall], nno = a.mid ? 0 : a.start[NS_NORM][a.nbig], apart = nno > 512 || !nsm;
     if (nsm) {
         hipLaunchKernelGGL(ns_first_kernel, dim3(nsm + (apart ? 0 : nno)), dim3(256), 0, st, a, co, nsm);
         P2C_LAUNCH_CHECK();
@@ -757,6 +1179,16 @@ int ns_chunk(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, co
         P2C_LAUNCH_CHECK();
     }
     if (!a.nbig) return P2C_OK;
+    if (a.mid) {
+        int most = 0;
+        for (int i = 0; i < a.nbig; ++i) most = a.mat[i].mP * a.mat[i].nP > most ? a.mat[i].mP * a.mat[i].nP : most;
+        const int lds = 2 * most * 4 + 64;
+        const hipError_t rc = hipFuncSetAttribute((const void *)ns_mid_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NS_MID * 4 + 64);
+        if (rc != hipSuccess) return (int)rc;
+        hipLaunchKernelGGL(ns_mid_kernel, dim3(a.start[NS_ALL][a.nbig]), dim3(512), lds, st, a, co);
+        P2C_LAUNCH_CHECK();
+        return P2C_OK;
+    }
     hipLaunchKernelGGL(ns_begin_kernel, dim3(a.start[NS_TILES][a.nbig]), dim3(256), 0, st, a);
     P2C_LAUNCH_CHECK();
     const NsTab *tab = (const NsTab *)ws;

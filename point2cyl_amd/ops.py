@@ -1618,7 +1618,7 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
             src, dst = (g, o) if g.dim() == 2 else (g.reshape(-1, *g.shape[-2:]), o.view(-1, *g.shape[-2:]))
             # (bound to `src` until the launch: reshape may have made a copy)
             groups.setdefault(_DTYPES[g.dtype], []).append((src, _ns_record(src, dst)))
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         for dt, recs in groups.items():
             buf = b"".join(r for _, r in recs)
             mats = ctypes.cast(ctypes.c_char_p(buf), ctypes.POINTER(_lib.NsMatrix))
@@ -1632,26 +1632,30 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
 class Int8Rows:
     """Rows in 8 bits: `q` (M, K) int8 and `scale` (M,) fp32, x ~ q * scale[:, None].  `q` is a view of rows padded to a multiple of 64 bytes with
     zeros (what the products read)."""
-    __slots__ = ("store", "scale", "q")
+    __slots__ = ("store", "scale", "K")
 
     def __init__(self, store, scale, K):
-        self.store, self.scale, self.q = store, scale, store[:, :K]
+        self.store, self.scale, self.K = store, scale, K
+
+    @property
+    def q(self):
+        return self.store[:, :self.K]
 
     @property
     def shape(self):
-        return self.q.shape
+        return torch.Size((self.store.shape[0], self.K))
 
     @property
     def device(self):
-        return self.q.device
+        return self.store.device
 
     def dequantize(self, dtype=torch.float32):
         """q * scale as (M, K) of `dtype`."""
         if dtype not in _DTYPES:
             raise TypeError("dequantize gives fp32, bf16 or fp16, not %s" % dtype)
-        M, K = self.q.shape
+        M, K = self.shape
         out = torch.empty(M, K, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
+        with _lib.on(self.device):
             call("p2c_dequantize_rows", ptr(self.store), ptr(self.scale), M, K, self.store.shape[1], ptr(out), _DTYPES[dtype], stream())
         return out
 
@@ -1665,7 +1669,7 @@ def _int8_rows_in(x, what):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad() or on a detached tensor" % what)
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
         raise ValueError("%s takes rows (M, K) with K of 1 ... 131072, got %s" % (what, tuple(x.shape)))
-    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.stride(0) >= 0 else x.contiguous()
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def quantize_rows(x):
@@ -1677,7 +1681,7 @@ def quantize_rows(x):
     Kp = (K + 63) // 64 * 64
     q = torch.empty(M, Kp, dtype=torch.int8, device=x.device)
     scale = torch.empty(M, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on(x.device):
         call("p2c_quantize_rows", ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K, M, K, Kp, ptr(q), ptr(scale), stream(),
              nbytes=float(M) * (K * x.element_size() + Kp))
     return Int8Rows(q, scale, K)
@@ -1702,7 +1706,7 @@ class Int8Weight:
         self.Kp, Np = (self.K + 63) // 64 * 64, (self.N + 255) // 256 * 256
         self.q = torch.zeros(Np, self.Kp, dtype=torch.int8, device=dev)
         self.scale = torch.zeros(Np, dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             call("p2c_quantize_rows", ptr(w), _DTYPES[w.dtype], w.stride(0) if self.N > 1 else self.K, self.N, self.K, self.Kp, ptr(self.q), ptr(self.scale), stream())
         self.bias = None
         if bias is not None:
@@ -1757,8 +1761,8 @@ def linear_int8(x, w, act="none", beta=100.0, threshold=20.0, add=None, out_dtyp
         ldadd = add.stride(0) if M > 1 else w.N
     epi = (ptr(w.q), ptr(w.scale), ptr(w.bias), ptr(add), ldadd, _INT8_ACTS[act], float(beta), float(threshold))
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        if requantize and L.p2c_int8_requant_supported(w.N):
+    with _lib.on(dev):
+        if requantize and L.p2c_int8_requant_supported(w.N, _INT8_ACTS[act], float(threshold)):
             rows = rows or quantize_rows(x)
             ldo = (w.N + 63) // 64 * 64
             q = torch.empty(M, ldo, dtype=torch.int8, device=dev)

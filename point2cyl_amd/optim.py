@@ -169,7 +169,7 @@ class Muon(Adam):
             rest = [p for p in ps if p.dim() < 2] if group["use_muon"] else ps
             if mats:
                 _lib.require_device(*mats)
-                with torch.cuda.device(mats[0].device):
+                with _lib.on(mats[0].device):
                     _, rec, n, nb, co, _ = self._matrices(gi, mats, group)
                     if n:
                         if self._ws is None or self._ws.numel() < nb or self._ws.device != mats[0].device:

@@ -357,7 +357,12 @@ def test_linear_int8_requantized(M, K, N, act, with_add):
     assert h.shape == (M, N) and not h.store[:, N:].any()
     top = y32.abs().amax(1)
     s = top * torch.tensor(1.0 / 127.0, device="cuda")
-    assert ((h.scale - s).abs() <= 2.0 ** -20 * s + 1e-30).all()                     # the epilogues may order their roundings differently
+    # the epilogues may order their roundings differently: 2^-20 of the largest value.  Where a softplus' largest argument z is negative its value is
+    # exp(beta z) / beta, whose relative error is beta |z| times that of z (d log f / d log z = beta z): both sides carry 2^-22 beta |z| more
+    amp = 1.0
+    if act == "softplus":
+        amp = 1.0 + 100.0 * (-linear64(*rows64(x), *rows64(W), b, add)[0].amax(1)).clamp_min(0.0).float()
+    assert ((h.scale - s).abs() <= 2.0 ** -20 * amp * s + 1e-30).all()
     back = h.q.double() * h.scale.double()[:, None]
     assert ((back - want).abs() <= tol + h.scale.double()[:, None] * 0.5001).all()   # half a quantum
 

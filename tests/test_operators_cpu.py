@@ -33,9 +33,9 @@ def test_newton_schulz_entry_refuses_bad_arguments():
     assert L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, co, 0.0, ONE, big, None) == -1
     assert L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, co, float("nan"), ONE, big, None) == -1
     assert L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, None, 1e-7, ONE, big, None) == -1
-    need = L.p2c_newton_schulz_ws_bytes(_mats((64, 64)), 1)
-    assert need > 0 and L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, co, 1e-7, ONE, need - 1, None) == -1   # workspace too small
-    assert L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, co, 1e-7, ctypes.c_void_p(8), big, None) == -1       # ... or not aligned
+    need = L.p2c_newton_schulz_ws_bytes(_mats((100, 300)), 1)
+    assert need > 0 and L.p2c_newton_schulz(_mats((100, 300)), 1, 0, 5, co, 1e-7, ONE, need - 1, None) == -1   # workspace too small
+    assert L.p2c_newton_schulz(_mats((100, 300)), 1, 0, 5, co, 1e-7, ctypes.c_void_p(8), big, None) == -1       # ... or not aligned
     wild = (ctypes.c_float * 15)(*([10.0, 20.0, 30.0] * 5))
     assert L.p2c_newton_schulz(_mats((64, 64)), 1, 0, 5, wild, 1e-7, ONE, big, None) == -1
     nan = (ctypes.c_float * 15)(*([float("nan")] * 15))
@@ -51,7 +51,8 @@ def test_int8_entries_refuse_bad_arguments():
     assert L.p2c_int8_padded(1) == 64 and L.p2c_int8_padded(64) == 64 and L.p2c_int8_padded(65) == 128 and L.p2c_int8_padded(0) == 0
     assert L.p2c_int8_padded_out(1) == 256 and L.p2c_int8_padded_out(257) == 512
     assert L.p2c_int8_few_supported(32, 2048) == 1 and L.p2c_int8_few_supported(33, 8) == 0 and L.p2c_int8_few_supported(1, 2049) == 0
-    assert L.p2c_int8_requant_supported(512) == 1 and L.p2c_int8_requant_supported(513) == 0
+    assert L.p2c_int8_requant_supported(512, 2, 20.0) == 1 and L.p2c_int8_requant_supported(513, 0, 20.0) == 0
+    assert L.p2c_int8_requant_supported(8, 2, 5.0) == 0 and L.p2c_int8_requant_supported(8, 1, 5.0) == 1
     q = lambda **k: L.p2c_quantize_rows(*[dict(x=ONE, dt=0, ld=8, M=2, K=8, Kp=64, q=ONE, s=ONE, st=None, **{})[n] if n not in k else k[n]  # noqa: E731
                                           for n in ("x", "dt", "ld", "M", "K", "Kp", "q", "s", "st")])
     assert q(M=0) == 0                                             # no rows: no launch

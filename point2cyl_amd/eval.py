@@ -365,6 +365,8 @@ def build_parser():
     for f in ("norm_eig", "add_noise", "use_gt_normals", "use_gt_segmentation", "use_gt_bb", "with_sketch_fit"):
         p.add_argument("--" + f, action="store_true")
     p.add_argument("--noise_sigma", type=float, default=0.01)
+    p.add_argument("--int8_decoder", action="store_true", help="with --with_sketch_fit: the profile decoder's hidden products in 8-bit integers "
+                   "(implicit.Int8ImplicitNet); the two fitting losses then carry its quantisation, the other metrics are untouched")
     p.add_argument("--im_logdir", default="./results/IGR_dense/", type=str)
     p.add_argument("--im_ckpt", default="latest.pth", type=str)
     p.add_argument("--synthetic", type=int, default=0, help="evaluate N generated extrusion-cylinder clouds instead of <data_dir>/<split>.h5")
@@ -386,6 +388,8 @@ def build_parser():
 def main(argv=None):
     a = build_parser().parse_args(argv)
     hostmem.setup_cli()        # large host blocks stay mapped after free; torch's CPU pool sized to the cgroup's CPU quota (hostmem.py)
+    if a.int8_decoder and not a.with_sketch_fit:
+        raise SystemExit("--int8_decoder changes the decoder of --with_sketch_fit: it needs that flag")
     if not torch.cuda.is_available():
         raise SystemExit("point2cyl_amd.eval needs an MI355X (HIP) device; there is no CPU path")
     from . import ddp, synth
@@ -428,6 +432,9 @@ def main(argv=None):
             pn_encoder.load_state_dict(ck["encoder_state_dict"])
         implicit_net.to(dev).eval()
         pn_encoder.to(dev).eval()
+        if a.int8_decoder:
+            from .implicit import Int8ImplicitNet
+            implicit_net = Int8ImplicitNet(implicit_net)
     acc = Accumulator(("pred_fit_cyl_loss", "pred_fit_glob_loss") if a.with_sketch_fit else ())
     os.makedirs(a.dump_dir, exist_ok=True)
     log = open(os.path.join(a.dump_dir, "log_evaluate.txt" if world == 1 else "log_evaluate.%d.txt" % rank), "w")

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, ops
 from ._lib import call, ptr, stream
 
 
@@ -361,6 +361,54 @@ class ImplicitNet(nn.Module):
                 else:
                     x = F.relu(x)
         return x[:, :N] if Np != N else x
+
+
+class Int8ImplicitNet:
+    """An ImplicitNet for evaluation with its hidden products in 8-bit integers (ops.linear_int8: a scale per row and per output channel), e.g. for
+    the fitting losses over all points (eval.py:555-590: clouds x profiles x points rows through eight 512-wide layers).  The activations go from
+    one hidden layer to the next in 8 bits.  What reads the point's coordinates - the first layer and the input block of a skip layer - and the
+    last layer (a single output) stay in the 32-bit kernels: in 8 bits a coordinate would be a step of 1 / 127 of the code beside it.
+
+    The weights are taken over when it is built: build it again after the network changed.  No gradient; the result is fp32 (M, 1)."""
+
+    def __init__(self, net):
+        d_in = net.lin0.weight.shape[1]
+        _lib.require_device(net.lin0.weight)
+        lay = _decoder_layout(net, d_in)
+        if len(lay) < 3:
+            raise ValueError("Int8ImplicitNet: a network of %d layers has no hidden product" % len(lay))
+        self.d_in, self.beta = d_in, float(net.beta)
+        self.first, self.last = (lay[0][0], lay[0][2]), (lay[-1][0], lay[-1][1], lay[-1][2], lay[-1][3])
+        self.hidden, prev = [], lay[0][3]
+        for Wa, Wb, b, N, Np in lay[1:-1]:
+            self.hidden.append((ops.Int8Weight(Wa[:N, :prev], b[:N]), Wb, N))
+            prev = N
+
+    @torch.no_grad()
+    def __call__(self, input):
+        if not input.is_cuda:
+            raise RuntimeError("point2cyl_amd.implicit.Int8ImplicitNet runs on the HIP device only (got %s); there is no CPU path" % input.device)
+        if input.dim() != 2 or input.shape[1] != self.d_in:
+            raise ValueError("Int8ImplicitNet takes rows (M, %d), got %s" % (self.d_in, tuple(input.shape)))
+        M = input.shape[0]
+        if M == 0:
+            return torch.empty(0, self.last[3], dtype=torch.float32, device=input.device)
+        inp = _c(F.pad(input, (0, (-self.d_in) % 4)) if self.d_in % 4 else input)
+        sp = (self.beta, 20.0) if self.beta > 0 else None
+        x = _prod_nt(inp, *self.first, sp=sp)
+        if sp is None:
+            x = F.relu_(x)
+        x = x[:, :self.hidden[0][0].K]
+        for k, (w, Wb, N) in enumerate(self.hidden):
+            add = _prod_nt(inp, Wb)[:, :N] if Wb is not None else None
+            x = ops.linear_int8(x, w, act="softplus" if self.beta > 0 else "relu", beta=self.beta if self.beta > 0 else 1.0, add=add,
+                                **(dict(requantize=True) if k + 1 < len(self.hidden) else dict(out_dtype=torch.float32)))
+        Wa, Wb, b, N = self.last
+        pad = Wa.shape[1] - x.shape[1]
+        y = _prod_nt(_c(F.pad(x, (0, pad)) if pad else x), Wa, b)
+        if Wb is not None:
+            y = y + _prod_nt(inp, Wb)
+        return y[:, :N]
 
 
 class NormalPerPoint:

@@ -179,3 +179,28 @@ class Muon(Adam):
             if rest:
                 self._adam(gi, rest, group["lr"], group["betas"], group["adam_eps"])
         return loss
+
+
+def add_arguments(p):
+    """The trainers' flags for the choice of the update rule."""
+    p.add_argument("--optimizer", choices=("adam", "muon"), default="adam", help="muon: orthogonalised momentum for the weight matrices (optim.Muon), Adam "
+                   "for biases, BatchNorm and the output heads; the learning rates mean the same")
+    p.add_argument("--muon_momentum", type=float, default=0.95)
+    p.add_argument("--weight_decay", type=float, default=0.0, help="decoupled decay of the matrices (--optimizer muon only)")
+
+
+def from_arguments(a, groups, heads=()):
+    """The trainers' optimizer from their flags: groups = [{"params": [...], "lr": ...}, ...]; heads: parameters of output layers, whose rows
+    are separate regressions and not one operator - muon leaves them to Adam, in a group of their own behind the one they came from."""
+    if a.optimizer == "adam":
+        if a.weight_decay:
+            raise SystemExit("--weight_decay belongs to --optimizer muon (the reference's Adam has none)")
+        return Adam(groups)
+    out, ids = [], {id(p) for p in heads}
+    for k, g in enumerate(groups):                           # "source": a schedule of group k moves every part of it
+        ps = list(g["params"])
+        out.append({**g, "params": [p for p in ps if id(p) not in ids], "source": k})
+        own = [p for p in ps if id(p) in ids]
+        if own:
+            out.append({**g, "params": own, "use_muon": False, "source": k})
+    return Muon(out, momentum=a.muon_momentum, weight_decay=a.weight_decay)

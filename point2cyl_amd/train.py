@@ -69,6 +69,7 @@ def build_parser():
     p.add_argument("--max_steps", type=int, default=0, help="stop after this many optimizer steps (0: run all epochs)")
     p.add_argument("--quiet", action="store_true", help="no per-batch log line (each costs a device synchronisation)")
     p.add_argument("--report", type=str, default="", help="write a JSON throughput / loss report here at the end")
+    optim.add_arguments(p)
     return p
 
 
@@ -220,7 +221,8 @@ def _main(a, rank, world, local, dev, stream):
         ds = torch.utils.data.Subset(ds, range(lo, hi))
     data = ResidentDataset(ds, dev, a.num_point, subsample)
     B = min(a.batch_size, len(data))
-    opt = optim.Adam(model.parameters(), lr=a.learning_rate)    # train…:204; one launch for all 123 tensors (point2cyl_amd/optim.py)
+    # train…:204: Adam, one launch for all 123 tensors (point2cyl_amd/optim.py); --optimizer muon: the update rule beside it
+    opt = optim.from_arguments(a, [{"params": list(model.parameters()), "lr": a.learning_rate}], heads=list(model.fc2.parameters()))
     sync = ddp.FlatGradSync(model.parameters(), world)
     if a.no_graph:
         from . import autograph

@@ -83,6 +83,7 @@ def build_parser():
     p.add_argument("--no_graph", action="store_true", help="launch every kernel of the step from Python (and draw the projections' barrel samples on the "
                    "CPU generator, as the reference does) instead of replaying a HIP graph")
     p.add_argument("--report", type=str, default="")
+    optim.add_arguments(p)
     return p
 
 
@@ -143,7 +144,7 @@ def _main(a, rank, world, dev):
         groups.append({"params": list(model.parameters()), "lr": a.learning_rate})                           # :298-311
     if a.is_im_train:
         groups.append({"params": list(pn_encoder.parameters()), "lr": step_lr(0.001, 1000, 0.5, 0)})
-    opt = optim.Adam(groups)
+    opt = optim.from_arguments(a, groups, heads=list(model.fc2.parameters()))
     log = None
     if rank == 0:
         os.makedirs(a.logdir, exist_ok=True)
@@ -379,7 +380,9 @@ def _main(a, rank, world, dev):
         # the staircases count SAMPLES: under data parallelism a step consumes world * B of them (as point2cyl_amd.train does)
         lr = step.get_learning_rate(a.learning_rate, gstep, B * world, a.decay_step, a.decay_rate)     # :703-706: group 0 only
         if old_lr != lr:
-            opt.param_groups[0]["lr"] = lr
+            for gi, g in enumerate(opt.param_groups):          # (--optimizer muon holds a group's heads apart)
+                if g.get("source", gi) == 0:
+                    g["lr"] = lr
             old_lr = lr
         row = run_step(mom_fwd, eager=gstep == 0)          # (the first step's momentum differs from every later one: not worth a capture)
         mom_fwd = step.get_batch_norm_decay(gstep, B * world, a.bn_decay_step)                        # :698-701 (reaches the next forward)

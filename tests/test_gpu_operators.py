@@ -8,6 +8,9 @@ the 64-bit iterates, plus half a unit of the output type.  8-bit: the whole-numb
 six 32-bit roundings (2^-21 of the sum of magnitudes), the fast exponential and logarithm 2^-20 of the softplus' range, then half a unit of the
 output type."""
 import copy
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -488,3 +491,107 @@ def test_operators_on_another_stream_and_in_a_graph():
     for _ in range(4):
         o2.step()
     assert torch.equal(p, p2) and torch.equal(q, q2)
+
+
+# ------------------------------------------------------------------------------------------ the paths that use them
+def decoder64(net, x):
+    """The 8-bit decoder from its definition: hidden products of quantised rows and weights in 64 bits."""
+    L = net.num_layers - 1
+    h = None
+    for l in range(L):
+        lin = getattr(net, "lin%d" % l)
+        W, b = lin.weight.detach(), lin.bias.detach()
+        if l == 0:
+            z = x.double() @ W.double().t() + b.double()
+        elif l == L - 1:
+            return h @ W.double().t() + b.double()
+        else:
+            k = h.shape[1]
+            if l in net.skip_in:
+                W = W / 2 ** 0.5
+            z, _ = linear64(*rows64(h.float()), *rows64(W[:, :k].contiguous()), b)
+            if l in net.skip_in:
+                z = z + x.double() @ W[:, k:].double().t()
+        h = act64(z, "softplus" if net.beta > 0 else "relu", net.beta)
+
+
+@pytest.mark.parametrize("d_in,dims,skip,beta,M", [(258, [512] * 8, (4,), 100, 4099), (6, [64, 40, 48], (2,), 100, 300), (258, [512] * 8, (4,), 100, 7), (10, [33, 600, 31], (), 0, 70)])
+def test_int8_decoder(d_in, dims, skip, beta, M):
+    """implicit.Int8ImplicitNet against the decoder's definition with quantised hidden layers.  Both quantise activations that differ by 32-bit
+    roundings, so a few of them (2^-17 of the quotients lie that near to a half) end one step apart; such a step is 1 / 254 of the row's largest
+    activation and passes through the remaining layers.  A row is therefore either equal to 2^-14 of the outputs' size or a step apart somewhere:
+    most are equal, and none is further away than the quantisation moves the 32-bit decoder's output."""
+    from point2cyl_amd import implicit
+    torch.manual_seed(17)
+    net = implicit.ImplicitNet(d_in=d_in, dims=dims, skip_in=skip, geometric_init=True, radius_init=1, beta=beta).cuda()
+    r = gen(18)
+    with torch.no_grad():
+        for p in net.parameters():
+            p.add_(0.02 * r(*p.shape))
+    x = r(M, d_in) * 0.3
+    q = implicit.Int8ImplicitNet(net)
+    y = q(x)
+    want, plain = decoder64(net, x), net(x).double()
+    assert y.shape == (M, 1) and y.dtype == torch.float32 and torch.equal(y, q(x))
+    size = plain.abs().max().item()
+    off = (y.double() - want).abs()
+    noise = (want - plain).abs().max().item()
+    assert off.max().item() <= 2.0 * noise + 2.0 ** -14 * size
+    assert (off <= 2.0 ** -14 * size).float().mean().item() >= 0.5
+    assert noise <= 0.2 * size
+    assert q(x[:0]).shape == (0, 1)
+    with pytest.raises(ValueError):
+        q(x[:, :-1])
+
+
+def test_trained_with_muon_evaluated_in_8_bits():
+    """A run of them together: a profile decoder's weights updated by Muon from its own gradients, then applied in 8 bits.  The update is checked against
+    the rule on the same gradients, the 8-bit decoder against the definition on the updated weights."""
+    from point2cyl_amd import implicit, optim
+    torch.manual_seed(19)
+    net = implicit.ImplicitNet(d_in=6, dims=[128] * 4, skip_in=(2,), geometric_init=True, radius_init=1, beta=100).cuda()
+    mats = [p for p in net.parameters() if p.dim() == 2]
+    opt = optim.Muon(net.parameters(), lr=1e-3)
+    ref = Muon64(mats, 1e-3, 0.95, True, 0.0, "rms")
+    r = gen(20)
+    x = r(4096, 6)
+    target = x[:, -2:].norm(dim=1, keepdim=True) - 1.0
+    for _ in range(3):
+        opt.zero_grad(set_to_none=True)
+        (net(x) - target).abs().mean().backward()
+        ref.step([p.grad for p in mats])
+        opt.step()
+    for p, w, tol in zip(mats, ref.p, ref.tol):
+        assert (p.detach().double() - w).norm().item() <= tol
+    q = implicit.Int8ImplicitNet(net)
+    y, want, plain = q(x), decoder64(net, x), net(x).detach().double()
+    assert (y.double() - want).abs().max() <= 2.0 * (want - plain).abs().max() + 2.0 ** -14 * plain.abs().max()
+
+
+def _run(*args):
+    """A command of the package in a process of its own (the trainers set process-wide switches)."""
+    o = subprocess.run([sys.executable, "-m", *args], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=110)
+    assert o.returncode == 0, o.stderr[-3000:]
+    return o.stdout
+
+
+@pytest.mark.parametrize("extra", [[], ["--no_graph"]])
+def test_trainers_with_muon(tmp_path, extra):
+    rep = tmp_path / "report.json"
+    _run("point2cyl_amd.train", "--pred_seg", "--pred_normal", "--pred_bb", "--synthetic", "4", "--batch_size", "2", "--num_point", "1024", "--num_epochs", "3", "--optimizer", "muon",
+         "--weight_decay", "0.01", "--quiet", "--logdir", str(tmp_path / "a"), "--report", str(rep), *extra)
+    sd = torch.load(tmp_path / "a" / "model.pth", weights_only=True)["model"]
+    assert rep.exists() and all(torch.isfinite(v).all() for v in sd.values())
+    _run("point2cyl_amd.train_sketch", "--pred_seg", "--pred_normal", "--pred_bb", "--is_pc_train", "--is_im_train", "--with_im_loss", "--synthetic", "2", "--batch_size", "1",
+         "--num_point", "1024", "--num_sk_point", "128", "--num_epochs", "2", "--optimizer", "muon", "--logdir", str(tmp_path / "b"), "--im_logdir", str(tmp_path / "none"), *extra)
+    sd = torch.load(tmp_path / "b" / "model.pth", weights_only=True)
+    assert all(torch.isfinite(v).all() for part in sd.values() for v in part.values())
+
+
+def test_evaluation_with_the_8_bit_decoder(tmp_path):
+    out = [_run("point2cyl_amd.eval", "--synthetic", "2", "--random_init", "--batch_size", "2", "--num_point", "1024", "--num_sk_point", "256", "--with_sketch_fit", "--im_logdir",
+                str(tmp_path / "none"), "--no_prefetch", "--dump_dir", str(tmp_path / "d"), *extra).splitlines() for extra in ([], ["--int8_decoder"])]
+    fit = [[float(l.split("=")[1]) for l in o if "fitting loss=" in l] for o in out]
+    assert len(fit[0]) == len(fit[1]) == 2 and all(v == v and abs(v) < 1e9 for f in fit for v in f)
+    rest = [[l for l in o if l.startswith("Mean ") and "fitting" not in l] for o in out]
+    assert len(rest[0]) >= 5 and rest[0] == rest[1]                                  # the other metrics do not change

@@ -100,3 +100,24 @@ def test_muon_refuses_bad_settings():
     o = optim.Muon([p])
     with pytest.raises(ValueError):
         o.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, 2))], "momentum": 2.0})
+
+
+def test_the_8_bit_decoder_flag_needs_the_decoder():
+    from point2cyl_amd import eval as ev
+    with pytest.raises(SystemExit, match="with_sketch_fit"):
+        ev.main(["--int8_decoder", "--synthetic", "2"])
+
+
+def test_trainer_flags_choose_the_update_rule():
+    p = train.build_parser()
+    net = torch.nn.Sequential(torch.nn.Linear(4, 3), torch.nn.Linear(3, 2))
+    groups = [{"params": list(net.parameters()), "lr": 0.5}]
+    a = p.parse_args([])
+    assert type(optim.from_arguments(a, groups)) is optim.Adam
+    with pytest.raises(SystemExit):
+        optim.from_arguments(p.parse_args(["--weight_decay", "0.1"]), groups)
+    a = p.parse_args(["--optimizer", "muon", "--weight_decay", "0.1", "--muon_momentum", "0.9"])
+    o = optim.from_arguments(a, groups, heads=list(net[1].parameters()))
+    assert type(o) is optim.Muon and [g["use_muon"] for g in o.param_groups] == [True, False] and [g["source"] for g in o.param_groups] == [0, 0]
+    assert all(g["lr"] == 0.5 and g["weight_decay"] == 0.1 and g["momentum"] == 0.9 for g in o.param_groups)
+    assert [len(g["params"]) for g in o.param_groups] == [2, 2]

@@ -9,12 +9,14 @@
 // 32-bit product at a third of the fp16 rate, 5 times the rate of the chip's 32-bit matrix instruction.  2^12 fits because every matrix of
 // the iteration is bounded by a small spectral norm (the host refuses coefficients that leave (0, 15)); what drops below the fp16 range is
 // < 2^-37 of one.
-// a X is added in the epilogue in 32 bits and not folded into the polynomial's diagonal: folded, the rounding of a + ... hits the weak
+// a X is added to the finished product in 32 bits and not folded into the polynomial's diagonal: folded, the rounding of a + ... hits the weak
 // directions (3.7e-5 against 1.3e-5 on a low-rank 512 x 512 gradient; 1.1e-5 for plain 32-bit arithmetic).
 //
-// Layout: X is kept twice, S = X [mP][nP] and T = X^T [nP][mP], so that all three products of a step are C[i][j] = sum_k P[i][k] Q[j][k] with
-// k contiguous: A = S S^T, B = bA + cA A^T, T' = aT + T B^T (A, B symmetric: only tiles on and above the diagonal are computed, the mirror image
-// is stored with them).  An element is 4 bytes, 8 consecutive k = 16 bytes of hi and 16 bytes of lo; sides are padded with zeros to the tile.
+// Layout: X is kept twice, S = X (rows mP, k nP) and T = X^T (rows nP, k mP), so that all three products of a step are C[i][j] = sum_k P[i][k] Q[j][k]:
+// A = S S^T, B = bA + cA A^T, T' = aT + T B^T (A, B symmetric: only tiles on and above the diagonal are computed, the mirror image
+// is stored with them).  An element is 4 bytes, 8 consecutive k = 16 bytes of hi and 16 bytes of lo; an image is cut into blocks of
+// 32 k, [k / 32][row][128 bytes]: what a tile needs of a block is one run of memory, and a 32 x 32 piece of a result is 4 KB of it.  Sides are padded
+// with zeros to the tile.
 // All matrices of a call go through each product together: one launch per product, whatever their number (the descriptors ride in the arguments of
 // the first launch: no copy from the host, capturable).  Matrices whose small side is <= 32 take ns_small: one workgroup each.
 #include "tile_dma.h"
@@ -201,13 +203,22 @@ __device__ __forceinline__ void ns_norm(const NsTab &a, int id, double *red)
     if (threadIdx.x == 0) reinterpret_cast<double *>(a.ws + d.ws + b * d.ws_bs)[part] = red[0] + red[1] + red[2] + red[3];
 }
 
-// tile t of the upper triangle of an nt x nt grid, row by row -> (i, j), j >= i
-__device__ __forceinline__ void ns_triangle(int t, int nt, int &i, int &j)
+// Tiles of a symmetric product that reach the diagonal or lie above it: rows of tiles i, of tile rows `tr` high and `tb` wide, nt of them across
+__host__ __device__ __forceinline__ int ns_sym_tiles(int side, int tr, int tb)
+{
+    const int q = tr / tb, rows = side / tr, nt = side / tb;
+    return rows * nt - q * (rows * (rows - 1) / 2);
+}
+// tile t of them, row by row -> (i, j)
+__device__ __forceinline__ void ns_triangle(int t, int nt, int q, int &i, int &j)
 {
     i = 0;
-    while (t >= nt - i) { t -= nt - i; ++i; }
-    j = i + t;
+    while (t >= nt - q * i) { t -= nt - q * i; ++i; }
+    j = q * i + t;
 }
+__host__ __device__ __forceinline__ int ns_tile_rows(int tile) { return tile == 96 ? 128 : tile; }
+__host__ __device__ __forceinline__ int ns_tile_cols(int tile) { return tile == 96 ? 64 : tile; }
+__host__ __device__ constexpr int ns_waves(int cols) { return cols == 32 ? 1 : 4; }
 
 // table and records, spread over a launch's threads
 __device__ __forceinline__ void ns_records(const NsTab &a)
@@ -219,13 +230,13 @@ __device__ __forceinline__ void ns_records(const NsTab &a)
         const bool sym = k < a.nsym;
         const int id = sym ? k : k - a.nsym, *start = a.start[sym ? NS_SYM : NS_ALL], tile = sym ? a.tsym : a.tall, mi = ns_find(start, a.nbig, id);
         const NsMat &d = a.mat[mi];
-        const int mt = d.mP / tile, per = sym ? mt * (mt + 1) / 2 : mt * (d.nP / tile);
+        const int tr = ns_tile_rows(tile), tb = ns_tile_cols(tile), mt = d.mP / tb, per = sym ? ns_sym_tiles(d.mP, tr, tb) : mt * (d.nP / tr);
         int t = ns_xcd_order(id - start[mi], start[mi + 1] - start[mi]);
         NsRec r;
         r.mi = mi; r.mP = d.mP; r.nP = d.nP;
         r.b = t / per;
         t -= r.b * per;
-        if (sym) ns_triangle(t, mt, r.ti, r.tj);
+        if (sym) ns_triangle(t, mt, tr / tb, r.ti, r.tj);
         else { r.ti = t / mt; r.tj = t - r.ti * mt; }
         r.w = (unsigned long long)(a.ws + d.ws + r.b * d.ws_bs);
         rec[k] = r;
@@ -265,25 +276,53 @@ __global__ void __launch_bounds__(256) ns_begin_kernel(const NsTab a)
 #pragma unroll
         for (int k = 0; k < 8; ++k) u[k] = x[r][c8 + k];
         ns_split8(u, hi, lo);
-        h16x8 *o = reinterpret_cast<h16x8 *>(R + ((size_t)(r0 + r) * cols + c0 + c8) * 4);
+        h16x8 *o = reinterpret_cast<h16x8 *>(R + ((size_t)((c0 + c8) >> 5) * rows + r0 + r) * 128 + (c8 & 31) * 4);
         o[0] = hi; o[1] = lo;
 #pragma unroll
         for (int k = 0; k < 8; ++k) u[k] = x[c8 + k][r];
         ns_split8(u, hi, lo);
-        o = reinterpret_cast<h16x8 *>(C + ((size_t)(c0 + r) * rows + r0 + c8) * 4);
+        o = reinterpret_cast<h16x8 *>(C + ((size_t)((r0 + c8) >> 5) * cols + c0 + r) * 128 + (c8 & 31) * 4);
         o[0] = hi; o[1] = lo;
     }
 }
 
-// ---- one product of a step for every matrix.  PH 1: A = S S^T.  2: B = b A + c A A^T.  3: T' = a T + T B^T (and S').  4: as 3, into the result.
-// Tile TB x TB, one wave of 32 x 32 (TB = 32) or four waves of TB/2 x TB/2 for each of KG groups that share the k range (group g takes k-tiles
-// g, g + KG, ...); k-tiles of 32 (128 bytes a row) in NST LDS stages filled by direct copies, one barrier per KG k-tiles.
-template <int TB, int KG, int NST, int PH>
-__global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(const NsTab *__restrict__ tab, const NsRec *__restrict__ recs, const float ca, const float cb, const int cur)
+// four values of a lane times a power of two as two fp16 each
+__device__ __forceinline__ void ns_split4(float v0, float v1, float v2, float v3, float f, h16x4 &hi, h16x4 &lo)
 {
-    constexpr int WG = TB == 32 ? 1 : 4, RB = 128, TILE = 2 * TB * RB, STAGE = KG * TILE, NT = TB == 128 ? 2 : 1, LPW = TILE / 1024 / WG;
+    const float v[4] = {v0, v1, v2, v3};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = (_Float16)(v[e] * f);
+        lo[e] = (_Float16)__builtin_fmaf(v[e], f, -(float)hi[e]);
+    }
+}
+
+// 4 x 4 half words across a quad of lanes: in, word e of lane q is M[e][q]; out, lane q holds M[q][0..3]
+__device__ __forceinline__ uint2 ns_quad_transpose(uint2 r, int lane)
+{
+    const uint32_t sel = lane & 1 ? 0x03020706u : 0x05040100u;             // odd: {high of the partner, own high}; even: {own low, low of the partner}
+    const uint32_t a0 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.x), r.x, sel), a1 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.y), r.y, sel);
+    const bool up = (lane & 2) != 0;
+    const uint32_t y = (uint32_t)p2c_dpp<0x4E>((int)(up ? a0 : a1));
+    return up ? make_uint2(y, a1) : make_uint2(a0, y);
+}
+
+// ---- one product of a step for every matrix.  PH 1: A = S S^T.  2: B = b A + c A A^T.  3: T' = a T + T B^T (and S').  4: as 3, into the result.
+// Tile TR x TB: 128 x 128 or 128 x 64 (four waves of 64 x 64 or 64 x 32), 64 x 64 (four of 32 x 32) or 32 x 32 (one), for each of KG groups that share
+// the k range (group g takes blocks g, g + KG, ...).  NST stages of one block (32 k, 128 bytes a row) are filled by direct copies, NST - 1 of them in flight.
+// A block is multiplied in two halves; the fragments of the next half are read, and the copies issued, BETWEEN the products of this one: instructions issue
+// in order, and copies in one go kept a wave from its products until the memory pipe had taken them (copies and products took the sum of their times;
+// 8 x 1024 x 2048: T' 136 us with reads, copies and products in turn, 123 with the reads a half ahead, 112 with the copies spread).
+// The addend b A, a T is the product's own first operand, so it is picked up when its block passes by: a product with the unit matrix, exact, into sums of
+// its own (into the product's it would be rounded again by every later step).  Fetched from memory in the results' layout it cost 10000 clocks a tile.
+// What bounds it at 8 x 1024 x 2048: the card's power.  T' runs 103 GFLOP in 115 us (900 TFLOP/s, against 1160 of a large library product) at 1.75 GHz;
+// the same launches on zeros take 24 us less.
+template <int TR, int TB, int KG, int NST, int PH>
+__global__ void __launch_bounds__(64 * ns_waves(TB) * KG, 2) ns_product_kernel(const NsTab *__restrict__ tab, const NsRec *__restrict__ recs, const float ca, const float cb, const int cur)
+{
+    constexpr int WG = ns_waves(TB), RB = 128, TILE = (TR + TB) * RB, STAGE = KG * TILE, NX = TR >= 128 ? 2 : 1, NY = TB / 64 < 1 ? 1 : TB / 64, LPW = TILE / 1024 / WG;
     constexpr int GP = 4 / KG;                      // row groups of a piece (8 g + 4 h + 0..3) that a k-group finishes
-    static_assert(KG == 1 || NT == 1, "");
+    static_assert(KG == 1 || NX * NY == 1, "");
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const NsRec d = recs[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 63, gw = __builtin_amdgcn_readfirstlane(tid >> 6), wave = gw % WG, kg = gw / WG, il = lane & 31, h = lane >> 5;
@@ -294,159 +333,175 @@ __global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(
     if (PH == 1) { P = Q = ns_S(w); K = d.nP; }
     else if (PH == 2) { P = Q = ns_A(w, d); K = d.mP; }
     else { P = ns_T(w, d, cur); Q = ns_B(w, d); K = d.mP; }
-    const long long ld = (long long)K * 4;
-    P += (long long)ti * TB * ld;
-    Q += (long long)tj * TB * ld;
-    const int KT = K / 32, IT = (KT + KG - 1) / KG;
+    const long long pb = (long long)(PH <= 2 ? d.mP : d.nP) * RB, qb = (long long)d.mP * RB;       // bytes of a block of 32 k
+    P += ti * TR * RB;
+    Q += tj * TB * RB;
+    const int KB = K / 32, IT = (KB + KG - 1) / KG;
+    const int wr = WG == 1 ? 0 : (wave >> 1) * (32 * NX), wc = WG == 1 ? 0 : (wave & 1) * (32 * NY);
 
-    const int wr = WG == 1 ? 0 : (wave >> 1) * (TB / 2), wc = WG == 1 ? 0 : (wave & 1) * (TB / 2);
-    const bool mirror = PH == 3 || (PH <= 2 && ti != tj);
-    char *o1 = PH == 1 ? ns_A(w, d) : PH == 2 ? ns_B(w, d) : ns_T(w, d, cur ^ 1);
-    char *o2 = PH == 3 || PH == 4 ? ns_S(w) : o1;
-    const char *old = PH == 2 ? ns_A(w, d) : ns_S(w);
-    const int ld1 = d.mP, ld2 = PH <= 2 ? d.mP : d.nP;
-    auto at2 = [&](int x, int y, int g) { return ((size_t)(tj * TB + wc + y * 32 + il) * ld2 + ti * TB + wr + x * 32 + 8 * g) * 4 + 8 * h; };
-    // the addend is fetched ahead of the operands: behind the sums it would be one more trip to memory at the kernel's end
-    h16x4 oldh[NT][NT][GP], oldl[NT][NT][GP];
-    if (PH != 1) {
+    f32x16 acc[NX][NY], own[NX][NY];
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+    for (int p = 0; p < NX; ++p)
 #pragma unroll
-            for (int y = 0; y < NT; ++y)
+        for (int q = 0; q < NY; ++q)
 #pragma unroll
-                for (int g = 0; g < GP; ++g) {
-                    const char *q = old + at2(x, y, kg * GP + g);
-                    oldh[x][y][g] = *reinterpret_cast<const h16x4 *>(q);
-                    oldl[x][y][g] = *reinterpret_cast<const h16x4 *>(q + 16);
+            for (int r = 0; r < 16; ++r) acc[p][q][r] = own[p][q][r] = 0.f;
+    // a block's rows are one run of memory, so a wave's copies are 1 KB pieces of it: a scalar base and one lane offset (odd pieces of a single wave: the other swizzle)
+    const unsigned lo = lane / 8 * RB + (((lane & 7) ^ p2c_tile_swz<RB>(wave * 8 + lane / 8)) << 4);
+    auto copy = [&](int it, int stage, int i) {     // piece i of this wave (past the end: the last block again, into a stage that is not multiplied: the count in flight stays exact)
+        constexpr int NP = TR * RB / 1024 / WG;
+        const int k = min(it * KG + kg, KB - 1), at = (wave + (i < NP ? i : i - NP) * WG) * 1024;
+        char *st = smem + stage * STAGE + kg * TILE + (i < NP ? 0 : TR * RB) + at;
+        const char *src = (i < NP ? P + k * pb : Q + k * qb) + at;
+        __builtin_amdgcn_global_load_lds((p2c_glb_ptr)(src + (WG == 1 && (i & 1) ? lo ^ 64 : lo)), (p2c_lds_ptr)st, 16, 0, 0);
+    };
+    struct Frags { h16x8 p[NX][2], q[NY][2]; };
+    constexpr int M = 3 * NX * NY, R = 2 * (NX + NY);
+    auto read = [&](Frags &f, int stage, int half, int i) {                  // fragment i of R
+        const char *ps = smem + stage * STAGE + kg * TILE, *qs = ps + TR * RB;
+        const int pl = i / (NX + NY), x = i % (NX + NY), y = x - NX, c = 4 * half + 2 * h + pl;
+        if (x < NX) f.p[x][pl] = *reinterpret_cast<const h16x8 *>(ps + p2c_tile_at<RB>(wr + x * 32 + il, c));
+        else f.q[y][pl] = *reinterpret_cast<const h16x8 *>(qs + p2c_tile_at<RB>(wc + y * 32 + il, c));
+    };
+    // the reads of the next half go between the products of this one, two for each of the first; so do the copies, evenly
+    auto reads = [&](Frags &f, int stage, int half, int n) {
+#pragma unroll
+        for (int i = 2 * n; i < (n + 1 == M ? R : 2 * n + 2) && i < R; ++i) read(f, stage, half, i);
+    };
+    const int cy = (tj * TB + wc) >> 5;             // the k-tile of this wave's first 32 columns
+    // after product n: then(n)
+    auto multiply = [&](const Frags &f, int it, int half, auto then) {
+        const bool on = KG == 1 || it * KG + kg < KB;
+        const int k = it * KG + kg;
+#pragma unroll
+        for (int pr = 0; pr < 3; ++pr)              // small products first
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int y = 0; y < NY; ++y) {
+                    if (on) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[x][pr == 1], f.q[y][pr == 0], acc[x][y], 0, 0, 0);
+                    then((pr * NX + x) * NY + y);
                 }
-    }
-
-    f32x16 acc[NT][NT];
+        if (!on) return;
+        if (PH != 1) {
 #pragma unroll
-    for (int p = 0; p < NT; ++p)
+            for (int y = 0; y < NY; ++y)
+                if (k == cy + y) {
+                    h16x8 one;                      // the unit matrix' half of this step as a fragment
 #pragma unroll
-        for (int q = 0; q < NT; ++q)
+                    for (int e = 0; e < 8; ++e) one[e] = (_Float16)(16 * half + 8 * h + e == il ? 1.f : 0.f);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[p][q][r] = 0.f;
-
-#define P2C_NS_COPY(IT_)                                                                             \
-    do {                                                                                             \
-        const int k__ = min((IT_) * KG + kg, KT - 1);                                                \
-        char *st__ = smem + ((IT_) % NST) * STAGE + kg * TILE;                                       \
-        p2c_tile_copy<TB, RB, WG>(P + (long long)k__ * RB, ld, TB - 1, st__, wave, lane);            \
-        p2c_tile_copy<TB, RB, WG>(Q + (long long)k__ * RB, ld, TB - 1, st__ + TB * RB, wave, lane);  \
-    } while (0)
+                    for (int x = 0; x < NX; ++x)
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s) P2C_NS_COPY(s);
-    for (int it = 0; it < IT; ++it) {
-        p2c_tile_wait<(NST - 2) * LPW>();           // stage `it` is here, and nobody reads stage it - 1 any more
-        P2C_NS_COPY(it + NST - 1);                  // (past the end: the last tile again, into a stage that is never read: the count in flight stays exact)
-        if (KG > 1 && it * KG + kg >= KT) continue;
-        const char *ps = smem + (it % NST) * STAGE + kg * TILE, *qs = ps + TB * RB;
-        // every fragment of the k-tile is requested before the first product (left to itself the compiler waits for LDS three times per k-step)
-        h16x8 p[2][NT][2], q[2][NT][2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int pl = 0; pl < 2; ++pl) {
-                    const int c = (2 * s + h) * 2 + pl;
-                    p[s][x][pl] = *reinterpret_cast<const h16x8 *>(ps + p2c_tile_at<RB>(wr + x * 32 + il, c));
-                    q[s][x][pl] = *reinterpret_cast<const h16x8 *>(qs + p2c_tile_at<RB>(wc + x * 32 + il, c));
+                        for (int pl = 1; pl >= 0; --pl) own[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[x][pl], one, own[x][y], 0, 0, 0);
                 }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int pr = 0; pr < 3; ++pr)          // small products first
-#pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int y = 0; y < NT; ++y)
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[s][x][pr == 1], q[s][y][pr == 0], acc[x][y], 0, 0, 0);
-    }
-#undef P2C_NS_COPY
-    p2c_tile_wait<0>();                             // the surplus copies have landed: the stages are free
-
-    // ---- epilogue.  A lane holds column il of a 32 x 32 piece, rows 8 g + 4 h + (0..3): four consecutive k of the transposed image, which is
-    // read (the addend) and written from the registers; the straight image goes through LDS to get consecutive k per lane.
-    // one group g of four rows of piece (x, y): c = the sums; leaves the new values in c
-    auto finish = [&](int x, int y, int g, h16x4 oh, h16x4 ol, float (&c)[4]) {
-        if (PH == 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] *= NS_INV;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = __builtin_fmaf(ca, (float)oh[e] + (float)ol[e], cb * (c[e] * NS_INV));
-        }
-        if (mirror) {
-            h16x4 vh, vl;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                vh[e] = (_Float16)c[e];
-                vl[e] = (_Float16)(c[e] - (float)vh[e]);
-            }
-            char *o = o2 + at2(x, y, g);
-            *reinterpret_cast<h16x4 *>(o) = vh;
-            *reinterpret_cast<h16x4 *>(o + 16) = vl;
         }
     };
-    // a 32 x 32 piece of the result: lanes run along the contiguous side of the output
-    constexpr int LDS_ = PH == 4 ? 33 : 36;
-    auto last = [&](const float *stage, int x, int y, int first, int count) {
-        const NsMat &m = tab->mat[d.mi];
-        const int i0 = tj * TB + wc + y * 32, j0 = ti * TB + wr + x * 32;
-        for (int e0 = first; e0 < 1024; e0 += 4 * count) {
-            float o[4];
-            auto i = [&](int q) { const int e = e0 + q * count; return m.tall ? e & 31 : e >> 5; };
-            auto j = [&](int q) { const int e = e0 + q * count; return m.tall ? e >> 5 : e & 31; };
 #pragma unroll
-            for (int q = 0; q < 4; ++q) o[q] = stage[j(q) * LDS_ + i(q)] * NS_INV;
-            ns_store_n(*tab, m, d.b, o, [&](int q) { return i0 + i(q); }, [&](int q) { return j0 + j(q); });
+    for (int it = 0; it < NST; ++it)
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) copy(it, it, i);
+    Frags f0, f1;
+    int now = 0;                                    // stage of block it
+    p2c_tile_wait<(NST - 1) * LPW>();
+#pragma unroll
+    for (int i = 0; i < R; ++i) read(f0, 0, 0, i);
+    for (int it = 0; it < IT; ++it) {
+        const int next = now + 1 == NST ? 0 : now + 1;
+        __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);          // f0 has arrived (lgkmcnt 0): known before the next reads are issued, or the products would wait for those
+        multiply(f0, it, 0, [&](int n) {
+            reads(f1, now, 1, n);
+            asm volatile("" ::: "memory");          // (read here, not where they are used)
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        p2c_tile_wait<(NST - 2) * LPW>();           // block it + 1 is here; everybody has read block it
+        // issued in one go, the copies held up the wave and its products with it: 123 us instead of 112 for a T' of 8 x 1024 x 2048
+        multiply(f1, it, 1, [&](int n) {
+            reads(f0, next, 0, n);
+#pragma unroll
+            for (int i = n * LPW / M; i < (n + 1) * LPW / M; ++i) copy(it + NST, now, i);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        now = next;
+    }
+    p2c_tile_wait<0>();                             // the surplus copies have landed: the stages are free
+
+    // ---- epilogue.  A lane holds column il of a 32 x 32 piece, rows 8 g + 4 h + (0..3): four consecutive k of the transposed image as they are, of the straight one
+    // after a 4 x 4 exchange in the lane's quad.  Both images of a piece are put together in LDS and leave as whole 128-byte lines.
+    const bool mirror = PH == 3 || (PH <= 2 && tj * TB >= (ti + 1) * TR);       // (the tiles over the diagonal cover both sides of it)
+    char *o1 = PH == 1 ? ns_A(w, d) : PH == 2 ? ns_B(w, d) : ns_T(w, d, cur ^ 1);
+    char *o2 = PH == 3 ? ns_S(w) : o1;
+    const int rows1 = PH <= 2 ? d.mP : d.nP;
+    constexpr int LDF = 33;                         // floats of a staged row of the result
+    char *piece = smem + (KG == 1 ? 0 : KG * WG * 4 * 64 * 16) + wave * 8192;
+    auto finish = [&](int g, const float (&c)[4]) { // c: the new values (scaled), or the result
+        if (PH == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<float *>(piece)[(8 * g + 4 * h + e) * LDF + il] = c[e];
+        } else {
+            h16x4 hi, lo;
+            ns_split4(c[0], c[1], c[2], c[3], 1.0f, hi, lo);
+            const int at = p2c_tile_at<128>(il, 2 * g) + 8 * h;
+            *reinterpret_cast<h16x4 *>(piece + 4096 + at) = hi;
+            *reinterpret_cast<h16x4 *>(piece + 4096 + (at ^ 16)) = lo;
+            const uint2 th = ns_quad_transpose(__builtin_bit_cast(uint2, hi), lane), tl = ns_quad_transpose(__builtin_bit_cast(uint2, lo), lane);
+            const int at1 = p2c_tile_at<128>(8 * g + 4 * h + (lane & 3), (il >> 3) * 2) + (il & 4) * 2;
+            *reinterpret_cast<uint2 *>(piece + at1) = th;
+            *reinterpret_cast<uint2 *>(piece + (at1 ^ 16)) = tl;
+        }
+    };
+    // out: `first` of `count` lanes that share a piece; r0, c0: its place
+    auto leave = [&](int r0, int c0, int first, int count) {
+        if (PH == 4) {
+            const NsMat &m = tab->mat[d.mi];
+            const float *stage = reinterpret_cast<const float *>(piece);
+            for (int e0 = first; e0 < 1024; e0 += 4 * count) {                      // lanes run along the contiguous side of the output
+                float o[4];
+                auto i = [&](int q) { const int e = e0 + q * count; return m.tall ? e & 31 : e >> 5; };
+                auto j = [&](int q) { const int e = e0 + q * count; return m.tall ? e >> 5 : e & 31; };
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[q] = stage[j(q) * LDF + i(q)] * NS_INV;
+                ns_store_n(*tab, m, d.b, o, [&](int q) { return c0 + i(q); }, [&](int q) { return r0 + j(q); });
+            }
+        } else {
+#pragma unroll
+            for (int u = first; u < 256; u += count) {
+                const int r = u >> 3, p = u & 7, c = p ^ p2c_tile_swz<128>(r);
+                *reinterpret_cast<f32x4 *>(o1 + ((size_t)(c0 >> 5) * rows1 + r0 + r) * 128 + c * 16) = *reinterpret_cast<const f32x4 *>(piece + u * 16);
+                if (mirror) *reinterpret_cast<f32x4 *>(o2 + ((size_t)(r0 >> 5) * d.mP + c0 + r) * 128 + c * 16) = *reinterpret_cast<const f32x4 *>(piece + 4096 + u * 16);
+            }
         }
     };
     if (KG == 1) {
-        float *stage = reinterpret_cast<float *>(smem) + wave * (32 * 36);
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < NX; ++x)
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                const int r0 = ti * TB + wr + x * 32, c0 = tj * TB + wc + y * 32;
+            for (int y = 0; y < NY; ++y) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    float c[4] = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]};
-                    finish(x, y, g, oldh[x][y][g], oldl[x][y][g], c);
+                    float c[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) stage[(8 * g + 4 * h + e) * LDS_ + il] = c[e];
+                    for (int e = 0; e < 4; ++e)
+                        c[e] = PH == 1 ? acc[x][y][4 * g + e] * NS_INV : __builtin_fmaf(ca, own[x][y][4 * g + e], cb * (acc[x][y][4 * g + e] * NS_INV));
+                    finish(g, c);
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (PH == 4) {
-                    last(stage, x, y, lane, 64);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int u = lane + 64 * q, r = u >> 2, c8 = (u & 3) * 8;
-                        float v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = stage[r * LDS_ + c8 + k];
-                        h16x8 hi, lo;
-                        ns_split8(v, hi, lo);
-                        h16x8 *o = reinterpret_cast<h16x8 *>(o1 + ((size_t)(r0 + r) * ld1 + c0 + c8) * 4);
-                        o[0] = hi; o[1] = lo;
-                    }
-                }
+                leave(ti * TR + wr + x * 32, tj * TB + wc + y * 32, lane, 64);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
     } else {
-        // the groups' sums meet in LDS; group k finishes the rows 8 g + 4 h + (0..3), g = GP k ... GP k + GP - 1, of its wave's piece
+        // the groups' sums meet in LDS; group k finishes the row groups GP k ... GP k + GP - 1 of its wave's piece
         f32x4 *sums = reinterpret_cast<f32x4 *>(smem);                               // [group][wave][g][lane]
-        float *stage = reinterpret_cast<float *>(smem + KG * WG * 4 * 64 * 16) + wave * (32 * 36);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            sums[((kg * WG + wave) * 4 + g) * 64 + lane] = f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
+        for (int g = 0; g < 4; ++g) {
+            f32x4 c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                c[e] = PH == 1 ? acc[0][0][4 * g + e] * NS_INV : __builtin_fmaf(ca, own[0][0][4 * g + e], cb * (acc[0][0][4 * g + e] * NS_INV));
+            sums[((kg * WG + wave) * 4 + g) * 64 + lane] = c;
+        }
         __syncthreads();
-        const int r0 = ti * TB + wr, c0 = tj * TB + wc;
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
             float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -456,29 +511,10 @@ __global__ void __launch_bounds__((TB == 32 ? 64 : 256) * KG) ns_product_kernel(
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[e] += v[e];
             }
-            finish(0, 0, kg * GP + g, oldh[0][0][g], oldl[0][0][g], c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) stage[(8 * (kg * GP + g) + 4 * h + e) * LDS_ + il] = c[e];
+            finish(kg * GP + g, c);
         }
         __syncthreads();
-        if (PH == 4) {
-            last(stage, 0, 0, kg * 64 + lane, 64 * KG);
-        } else {
-#pragma unroll
-            for (int q = 0; q < GP; ++q) {
-                const int u = (q * KG + kg) * 64 + lane, r = u >> 3, c4 = (u & 7) * 4;      // four consecutive k per lane
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(stage + r * 36 + c4);
-                h16x4 vh, vl;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    vh[e] = (_Float16)v[e];
-                    vl[e] = (_Float16)(v[e] - (float)vh[e]);
-                }
-                char *o = o1 + ((size_t)(r0 + r) * ld1 + c0 + (c4 & ~7)) * 4 + (c4 & 4) * 2;
-                *reinterpret_cast<h16x4 *>(o) = vh;
-                *reinterpret_cast<h16x4 *>(o + 16) = vl;
-            }
-        }
+        leave(ti * TR + wr, tj * TB + wc, kg * 64 + lane, 64 * KG);
     }
 }
 
@@ -550,34 +586,16 @@ struct NsMidImage { int base, rows; };                          // offset in LDS
 __device__ __forceinline__ int ns_mid_at(const NsMidImage &m, int row, int k) { return m.base + (k >> 5) * (m.rows * 128) + p2c_tile_at<128>(row, (k & 31) >> 3 << 1); }
 
 // 16 values of a lane (rows 8 g + 4 h + 0..3 of a 32 x 32 piece, times a power of two) as 4 x 4 consecutive k of image row `row`, k-tile k0 / 32
-__device__ __forceinline__ void ns_mid_split4(const f32x16 &v, int g, float f, h16x4 &hi, h16x4 &lo)
-{
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        hi[e] = (_Float16)(v[4 * g + e] * f);
-        lo[e] = (_Float16)__builtin_fmaf(v[4 * g + e], f, -(float)hi[e]);
-    }
-}
 __device__ __forceinline__ void ns_mid_put(char *lds, const NsMidImage &m, int row, int k0, int h, const f32x16 &v, float f)
 {
     const int at = ns_mid_at(m, row, k0) + 8 * h;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         h16x4 hi, lo;
-        ns_mid_split4(v, g, f, hi, lo);
+        ns_split4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3], f, hi, lo);
         *reinterpret_cast<h16x4 *>(lds + (at ^ (32 * g))) = hi;
         *reinterpret_cast<h16x4 *>(lds + (at ^ (32 * g + 16))) = lo;
     }
-}
-
-// 4 x 4 half words across a quad of lanes: in, word e of lane q is M[e][q]; out, lane q holds M[q][0..3]
-__device__ __forceinline__ uint2 ns_quad_transpose(uint2 r, int lane)
-{
-    const uint32_t sel = lane & 1 ? 0x03020706u : 0x05040100u;             // odd: {high of the partner, own high}; even: {own low, low of the partner}
-    const uint32_t a0 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.x), r.x, sel), a1 = __builtin_amdgcn_perm((uint32_t)p2c_dpp<0xB1>((int)r.y), r.y, sel);
-    const bool up = (lane & 2) != 0;
-    const uint32_t y = (uint32_t)p2c_dpp<0x4E>((int)(up ? a0 : a1));
-    return up ? make_uint2(y, a1) : make_uint2(a0, y);
 }
 
 __global__ void __launch_bounds__(512) ns_mid_kernel(const NsTab a, const NsCoef co)
@@ -807,7 +825,7 @@ __global__ void __launch_bounds__(512) ns_mid_kernel(const NsTab a, const NsCoef
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     h16x4 hi, lo;
-                    ns_mid_split4(x[y], g, 1.0f, hi, lo);
+                    ns_split4(x[y][4 * g], x[y][4 * g + 1], x[y][4 * g + 2], x[y][4 * g + 3], 1.0f, hi, lo);
                     *reinterpret_cast<h16x4 *>(smem + (at ^ (32 * g))) = hi;
                     *reinterpret_cast<h16x4 *>(smem + (at ^ (32 * g + 16))) = lo;
                     const uint2 th = ns_quad_transpose(__builtin_bit_cast(uint2, hi), lane), tl = ns_quad_transpose(__builtin_bit_cast(uint2, lo), lane);
@@ -1042,8 +1060,10 @@ __global__ void __launch_bounds__(256) ns_first_kernel(const NsTab a, const NsCo
 inline int ns_pad(int v, int to) { return (v + to - 1) / to * to; }
 inline bool ns_is_small(const p2c_ns_matrix &m) { return (m.rows < m.cols ? m.rows : m.cols) <= NS_SMALL; }
 
-// Tile of a chunk's products: 128 keeps the matrix units busy (a wave reads 16 KB of operands for 24 instructions), 64 has four times the
-// workgroups and a shorter chain per workgroup.  The choice is made for the widest product (all tiles); the padding of the sides follows it.
+// Tile of a chunk's products: 128 keeps the matrix units busy (a wave reads 8 KB of operands for 12 instructions), 64 has four times the
+// workgroups and a shorter chain per workgroup.  The choice is made for the widest product (all tiles); the padding of the sides follows it.  The symmetric
+// products of a chunk on 128 take 128 x 64 (code 96), as they have half the tiles (8 x 1024 x 2048, 288 or 576 tiles: 81 and 48 us or 77 and 46; 2048 x 2048,
+// 4000 x 1000, ...: 93 or 72).  256 x 128 with eight waves measured the same as 128 x 128 within 2 % both ways.
 inline int ns_tile(const p2c_ns_matrix *mats, int n)
 {
     long long t128 = 0;
@@ -1076,16 +1096,17 @@ int ns_check(const p2c_ns_matrix *mats, int n)
     return P2C_OK;
 }
 
-template <int TB, int KG, int NST, int PH>
+template <int TR, int TB, int KG, int NST, int PH>
 int ns_product(const NsTab *tab, const NsRec *recs, int grid, float ca, float cb, int cur, hipStream_t st)
 {
-    constexpr int WG = TB == 32 ? 1 : 4, OUT = KG == 1 ? 4 * 32 * 36 * 4 : KG * WG * 4 * 64 * 16 + WG * 32 * 36 * 4, OPS = KG * 2 * TB * 128 * NST, LDS = OPS > OUT ? OPS : OUT;
+    constexpr int WG = ns_waves(TB), OUT = WG * 8192 + (KG == 1 ? 0 : KG * WG * 4 * 64 * 16), OPS = KG * (TR + TB) * 128 * NST,
+                  LDS = OPS > OUT ? OPS : OUT;
     static_assert(LDS <= 160 * 1024, "");
     if (LDS > 65536) {
-        const hipError_t rc = hipFuncSetAttribute((const void *)ns_product_kernel<TB, KG, NST, PH>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t rc = hipFuncSetAttribute((const void *)ns_product_kernel<TR, TB, KG, NST, PH>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (rc != hipSuccess) return (int)rc;
     }
-    hipLaunchKernelGGL((ns_product_kernel<TB, KG, NST, PH>), dim3(grid), dim3((TB == 32 ? 64 : 256) * KG), LDS, st, tab, recs, ca, cb, cur);
+    hipLaunchKernelGGL((ns_product_kernel<TR, TB, KG, NST, PH>), dim3(grid), dim3(64 * WG * KG), LDS, st, tab, recs, ca, cb, cur);
     P2C_LAUNCH_CHECK();
     return P2C_OK;
 }
@@ -1100,14 +1121,14 @@ inline int ns_pick(const NsTab &a, bool sym, int pad)
         const long long mt = a.mat[i].mP / 32, nt = a.mat[i].nP / 32;
         t32 += (sym ? mt * (mt + 1) / 2 : mt * nt) * a.mat[i].batch;
     }
-    return pad == 128 ? 128 : t32 <= 512 ? 32 : 64;
+    return pad == 128 ? (sym ? 96 : 128) : t32 <= 512 ? 32 : 64;
 }
 
 inline int ns_starts(NsTab &a, int phase, int tile)
 {
     for (int i = 0; i < a.nbig; ++i) {
-        const int mt = a.mat[i].mP / tile, nt = a.mat[i].nP / tile;
-        a.start[phase][i + 1] = a.start[phase][i] + (phase == NS_SYM ? mt * (mt + 1) / 2 : mt * nt) * a.mat[i].batch;
+        const int tr = ns_tile_rows(tile), tb = ns_tile_cols(tile), m = a.mat[i].mP, n = a.mat[i].nP;
+        a.start[phase][i + 1] = a.start[phase][i] + (phase == NS_SYM ? ns_sym_tiles(m, tr, tb) : (m / tb) * (n / tr)) * a.mat[i].batch;
     }
     return a.start[phase][a.nbig];
 }
@@ -1115,9 +1136,10 @@ inline int ns_starts(NsTab &a, int phase, int tile)
 template <int PH>
 int ns_product_any(const NsTab *tab, const NsRec *recs, int tile, int grid, float ca, float cb, int cur, hipStream_t st)
 {
-    if (tile == 128) return ns_product<128, 1, 2, PH>(tab, recs, grid, ca, cb, cur, st);
-    if (tile == 64) return ns_product<64, 1, 4, PH>(tab, recs, grid, ca, cb, cur, st);
-    return ns_product<32, 4, 4, PH>(tab, recs, grid, ca, cb, cur, st);
+    if (PH <= 2 && tile == 96) return ns_product<128, 64, 1, 3, PH <= 2 ? PH : 1>(tab, recs, grid, ca, cb, cur, st);
+    if (PH >= 3 && tile == 128) return ns_product<128, 128, 1, 2, PH >= 3 ? PH : 3>(tab, recs, grid, ca, cb, cur, st);
+    if (tile == 64) return ns_product<64, 64, 1, 3, PH>(tab, recs, grid, ca, cb, cur, st);
+    return ns_product<32, 32, 4, PH == 1 ? 3 : 2, PH>(tab, recs, grid, ca, cb, cur, st);
 }
 
 // the chunk's table (without ws); returns the bytes of workspace it needs

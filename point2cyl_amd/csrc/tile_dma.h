@@ -38,7 +38,9 @@ __device__ __forceinline__ void p2c_tile_copy(const char *src, long long ld, int
 template <int N>
 __device__ __forceinline__ void p2c_tile_wait()
 {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);         // (vmcnt N, lgkmcnt 0; as a builtin, so that the compiler knows what has arrived)
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }

@@ -209,9 +209,14 @@ __device__ __forceinline__ float i8_softplus2(float z, const I8Poly &k)
 // ---- the product.  Tile BM x BN, WR x WC waves, k-tiles of 64 bytes in NST LDS stages filled by direct copies.  The operands are handed to the
 // matrix instruction weights first: a lane then holds ONE row of x and 4 consecutive output channels at a time, so the channel scales are
 // registers, the row scale is one number, and a row's maximum is an in-lane affair.
+// A k-tile is multiplied in two halves; the reads of the next half and the copies of a later k-tile are issued between the products of this one, because
+// instructions issue in order and a wave behind a queue of copies does not multiply.  16384 x 4096 x 4096: 299 us with copies, reads and products in turn,
+// 270 so = 2040 TOP/s (a large library product without scales, bias or rounding: 2130).
 template <int BM, int BN, int WR, int WC, int NST>
 struct I8Tile {
-    static constexpr int RB = 64, NW = WR * WC, STAGE = (BM + BN) * RB, TM = BM / WR / 32, TN = BN / WC / 32, LPW = STAGE / 1024 / NW;
+    static constexpr int RB = 64, NW = WR * WC, STAGE = (BM + BN) * RB, TM = BM / WR / 32, TN = BN / WC / 32;
+    static constexpr int NXC = BM * RB / 1024 / NW, NWC = BN * RB / 1024 / NW, LPW = NXC + NWC;       // copies per wave and k-tile: of x, of w, both
+    static_assert(BM * RB % (1024 * NW) == 0 && BN * RB % (1024 * NW) == 0, "the same number of copies in every wave");
 
     // meanwhile(): what is done while the first operands are on their way
     template <class F>
@@ -225,53 +230,91 @@ struct I8Tile {
             for (int q = 0; q < TM; ++q)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[p][q][r] = 0;
-        auto copy = [&](int kt) {
-            const int k = min(kt, KT - 1);
-            char *st = smem + (kt % NST) * STAGE;
-            p2c_tile_copy<BM, RB, NW>((const char *)x + (long long)k * RB, ldx, lastx, st, wave, lane);
-            p2c_tile_copy<BN, RB, NW>((const char *)w + (long long)k * RB, ldw, lastw, st + BM * RB, wave, lane);
+        const char *sx[NXC], *sw[NWC];               // this lane's source of each of the wave's copies
+#pragma unroll
+        for (int i = 0; i < NXC; ++i) sx[i] = (const char *)x + p2c_tile_source<RB>(wave + i * NW, ldx, lastx, lane);
+#pragma unroll
+        for (int i = 0; i < NWC; ++i) sw[i] = (const char *)w + p2c_tile_source<RB>(wave + i * NW, ldw, lastw, lane);
+        auto copy = [&](int kt, int stage, int i) {  // (past the end: the last k-tile again, into a stage that is not multiplied: the count in flight stays exact)
+            const long long k = (long long)min(kt, KT - 1) * RB;
+            char *st = smem + stage * STAGE + wave * 1024;
+            if (i < NXC) p2c_tile_piece(sx[i] + k, st + i * NW * 1024);
+            else p2c_tile_piece(sw[i - NXC] + k, st + BM * RB + (i - NXC) * NW * 1024);
         };
 #pragma unroll
-        for (int s = 0; s < NST - 1; ++s) copy(s);
+        for (int s = 0; s < NST; ++s)
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) copy(s, s, i);
         meanwhile();
         const int wr = wave / WC * (BM / WR), wc = wave % WC * (BN / WC);
+        struct Frags { i32x4 x[TM], w[TN]; };
+        constexpr int R = TM + TN, M = TM * TN;
+        auto read = [&](Frags &f, int stage, int half, int i) {              // fragment i of R
+            const char *xs = smem + stage * STAGE, *ws = xs + BM * RB;
+            if (i < TM) f.x[i] = *reinterpret_cast<const i32x4 *>(xs + p2c_tile_at<RB>(wr + i * 32 + il, 2 * half + h));
+            else f.w[i - TM] = *reinterpret_cast<const i32x4 *>(ws + p2c_tile_at<RB>(wc + (i - TM) * 32 + il, 2 * half + h));
+        };
+        // a half's products; after each, its share of the next half's reads and of what else is to be issued
+        auto multiply = [&](const Frags &f, Frags &g, int stage, int half, auto then) {
+#pragma unroll
+            for (int p = 0; p < TN; ++p)
+#pragma unroll
+                for (int q = 0; q < TM; ++q) {
+                    const int n = p * TM + q;
+                    acc[p][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[p], f.x[q], acc[p][q], 0, 0, 0);
+#pragma unroll
+                    for (int i = 2 * n; i < (n + 1 == M ? R : 2 * n + 2) && i < R; ++i) read(g, stage, half, i);
+                    then(n);
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        };
+        Frags f0, f1;
+        int now = 0;
+        p2c_tile_wait<(NST - 1) * LPW>();
+#pragma unroll
+        for (int i = 0; i < R; ++i) read(f0, 0, 0, i);
         for (int kt = 0; kt < KT; ++kt) {
-            p2c_tile_wait<(NST - 2) * LPW>();
-            copy(kt + NST - 1);
-            const char *xs = smem + (kt % NST) * STAGE, *ws = xs + BM * RB;
-            i32x4 fx[2][TM], fw[2][TN];
+            const int next = now + 1 == NST ? 0 : now + 1;
+            __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);              // f0 has arrived (lgkmcnt 0): known before the next reads are issued, or the products would wait for those
+            multiply(f0, f1, now, 1, [](int) {});
+            p2c_tile_wait<(NST - 2) * LPW>();                               // k-tile kt + 1 is here; everybody has read kt
+            multiply(f1, f0, next, 0, [&](int n) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                for (int q = 0; q < TM; ++q) fx[s][q] = *reinterpret_cast<const i32x4 *>(xs + p2c_tile_at<RB>(wr + q * 32 + il, 2 * s + h));
-#pragma unroll
-                for (int p = 0; p < TN; ++p) fw[s][p] = *reinterpret_cast<const i32x4 *>(ws + p2c_tile_at<RB>(wc + p * 32 + il, 2 * s + h));
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int p = 0; p < TN; ++p)
-#pragma unroll
-                    for (int q = 0; q < TM; ++q) acc[p][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][p], fx[s][q], acc[p][q], 0, 0, 0);
+                for (int i = n * LPW / M; i < (n + 1) * LPW / M; ++i) copy(kt + NST, now, i);
+            });
+            now = next;
         }
         p2c_tile_wait<0>();
     }
 };
 
-// scales and biases of BN channels (they are padded that far; `behind`: bias of channels that do not exist) and scales of BM rows, into LDS behind the
-// operand stages
+// Scales and biases of BN channels (they are padded that far; `behind`: bias of channels that do not exist) and scales of BM rows, for the LDS behind
+// the operand stages.  load() before the operands' copies, put() after: a load behind them could only be waited for with all of them.
 template <int BM, int BN, int NT>
-__device__ __forceinline__ void i8_factors(const I8Epi &e, int m0, int n0, int M, int N, float *f, int tid, float unit, float behind)
-{
+struct I8Factors {
+    float sw[(BN + NT - 1) / NT], bi[(BN + NT - 1) / NT], sx;
+    __device__ __forceinline__ void load(const I8Epi &e, int m0, int n0, int M, int N, int tid, float behind)
+    {
 #pragma unroll
-    for (int c = 0; c < BN; c += NT)
-        if (BN % NT == 0 || c + tid < BN) {
-            f[c + tid] = e.sw[n0 + c + tid] * unit;
-            f[BN + c + tid] = n0 + c + tid >= N ? behind : e.bias ? e.bias[n0 + c + tid] * unit : 0.f;
-        }
-    if (BM >= NT || tid < BM) f[2 * BN + tid] = e.sx[min(m0 + tid, M - 1)];
-}
+        for (int c = 0; c < BN; c += NT)
+            if (BN % NT == 0 || c + tid < BN) {
+                sw[c / NT] = e.sw[n0 + c + tid];
+                bi[c / NT] = n0 + c + tid >= N ? behind : e.bias ? e.bias[n0 + c + tid] : 0.f;
+            }
+        if (BM >= NT || tid < BM) sx = e.sx[min(m0 + tid, M - 1)];
+    }
+    __device__ __forceinline__ void put(float *f, int tid, float unit) const
+    {
+#pragma unroll
+        for (int c = 0; c < BN; c += NT)
+            if (BN % NT == 0 || c + tid < BN) {
+                f[c + tid] = sw[c / NT] * unit;
+                f[BN + c + tid] = bi[c / NT] * unit;
+            }
+        if (BM >= NT || tid < BM) f[2 * BN + tid] = sx;
+    }
+};
 
 __device__ __forceinline__ void i8_store4(float *row, int c, int N, f32x4 v)
 {
@@ -300,8 +343,10 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_linear_kernel(const int8
     const int bm = blockIdx.x / nbn, bn = blockIdx.x - bm * nbn, m0 = bm * BM, n0 = bn * BN;
     float *fact = reinterpret_cast<float *>(smem + FACT);
     i32x16 acc[T::TN][T::TM];
+    I8Factors<BM, BN, 64 * WR * WC> fa;
+    fa.load(e, m0, n0, M, N, tid, 0.f);
     T::run(x + (long long)m0 * ldx, ldx, M - 1 - m0, w + (long long)n0 * Kp, Kp, BN - 1, Kp / 64, smem, wave, lane, acc,
-           [&]() { i8_factors<BM, BN, 64 * WR * WC>(e, m0, n0, M, N, fact, tid, 1.0f, 0.f); });
+           [&]() { fa.put(fact, tid, 1.0f); });
 
     // epilogue, 32 rows x 32 TN channels of a wave at a time: finished in the registers (a lane: one row, 4 consecutive channels), through LDS in the
     // output's type, out in 16-byte pieces along the rows.  What differs between calls is decided per piece, not per element.
@@ -379,8 +424,9 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_requant_kernel(const int
     const float unit = ACT == 2 ? e.beta * 1.44269504f : 1.0f;
     float *fact = reinterpret_cast<float *>(smem + FACT);
     i32x16 acc[T::TN][T::TM];
-    T::run(x + (long long)m0 * ldx, ldx, M - 1 - m0, w, Kp, BN - 1, Kp / 64, smem, wave, lane, acc,
-           [&]() { i8_factors<BM, BN, 64 * WR * WC>(e, m0, 0, M, N, fact, tid, unit, ACT == 2 ? -__builtin_inff() : 0.f); });
+    I8Factors<BM, BN, 64 * WR * WC> fa;
+    fa.load(e, m0, 0, M, N, tid, ACT == 2 ? -__builtin_inff() : 0.f);
+    T::run(x + (long long)m0 * ldx, ldx, M - 1 - m0, w, Kp, BN - 1, Kp / 64, smem, wave, lane, acc, [&]() { fa.put(fact, tid, unit); });
 
     int8_t *qt = reinterpret_cast<int8_t *>(smem);                           // [BM][LDQ]
     float *rowtop = reinterpret_cast<float *>(smem + BM * LDQ);              // [WC][BM]
@@ -658,7 +704,9 @@ extern "C" int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx,
     if (!xq || !sx || !wq || !sw || !out) return P2C_EINVAL;
     if (((uintptr_t)xq & 15) || ((uintptr_t)wq & 15) || ldx % 16) return P2C_EALIGN;
     const hipStream_t st = (hipStream_t)stream;
-    if ((long long)p2c_cdiv(M, 256) * p2c_cdiv(N, 256) >= 192) return linear_any<256, 256, 2, 4, 4>(xq, ldx, wq, Kp, M, N, e, st);
+    // 256 x 256 reads each operand half as often as 128 x 128 (16384 x 4096 x 4096: 270 us against 384; 262144 x 512 x 512: 142 against 153), but has to
+    // fill most of the 256 CUs; the same limit for 128 x 128 against 64 x 64.
+    if ((long long)p2c_cdiv(M, 256) * p2c_cdiv(N, 256) >= 192) return linear_any<256, 256, 2, 4, 3>(xq, ldx, wq, Kp, M, N, e, st);
     if ((long long)p2c_cdiv(M, 128) * p2c_cdiv(N, 128) >= 192) return linear_any<128, 128, 2, 2, 3>(xq, ldx, wq, Kp, M, N, e, st);
     return linear_any<64, 64, 2, 2, 4>(xq, ldx, wq, Kp, M, N, e, st);
 }

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(64 * ns_waves(TB) * KG, 2) ns_product_kernel(c
         const int k = min(it * KG + kg, KB - 1), at = (wave + (i < NP ? i : i - NP) * WG) * 1024;
         char *st = smem + stage * STAGE + kg * TILE + (i < NP ? 0 : TR * RB) + at;
         const char *src = (i < NP ? P + k * pb : Q + k * qb) + at;
-        __builtin_amdgcn_global_load_lds((p2c_glb_ptr)(src + (WG == 1 && (i & 1) ? lo ^ 64 : lo)), (p2c_lds_ptr)st, 16, 0, 0);
+        p2c_tile_piece(src + (WG == 1 && (i & 1) ? lo ^ 64 : lo), st);
     };
     struct Frags { h16x8 p[NX][2], q[NY][2]; };
     constexpr int M = 3 * NX * NY, R = 2 * (NX + NY);

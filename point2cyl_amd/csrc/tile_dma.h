@@ -18,20 +18,18 @@ __device__ __forceinline__ int p2c_tile_swz(int r) { return (r / (256 / RB)) & (
 template <int RB>
 __device__ __forceinline__ int p2c_tile_at(int r, int c) { return r * RB + ((c ^ p2c_tile_swz<RB>(r)) << 4); }
 
-// Copies rows [0, R) x RB bytes with NW waves; `wave` must be wave-uniform.  src: first byte of row 0 at this k; rows past `last` are read from
-// row `last` (their results are never stored).  Every wave issues exactly R * RB / 1024 / NW copies.
-template <int R, int RB, int NW>
-__device__ __forceinline__ void p2c_tile_copy(const char *src, long long ld, int last, char *lds, int wave, int lane)
+// Piece `piece` of a tile is 1 KB of it: 1024 / RB rows.  The byte that lane `lane` fetches for it, counted from row 0 at this k; rows past `last` are
+// read from row `last` (their results are never stored).
+template <int RB>
+__device__ __forceinline__ long long p2c_tile_source(int piece, long long ld, int last, int lane)
 {
-    constexpr int ROWS = 1024 / RB, PIECES = R / ROWS;      // rows per instruction, instructions per tile
-    static_assert(PIECES % NW == 0, "the same number of copies in every wave");
-    const int r8 = lane / (RB / 16), p = lane & (RB / 16 - 1);
-#pragma unroll
-    for (int i = 0; i < PIECES / NW; ++i) {
-        const int piece = wave + i * NW, r = piece * ROWS + r8;
-        const char *g = src + (long long)min(r, last) * ld + ((p ^ p2c_tile_swz<RB>(r)) << 4);
-        __builtin_amdgcn_global_load_lds((p2c_glb_ptr)g, (p2c_lds_ptr)(lds + piece * 1024), 16, 0, 0);
-    }
+    const int r = piece * (1024 / RB) + lane / (RB / 16);
+    return (long long)min(r, last) * ld + (((lane & (RB / 16 - 1)) ^ p2c_tile_swz<RB>(r)) << 4);
+}
+// one copy of one wave; lds (the piece's place) must be wave-uniform
+__device__ __forceinline__ void p2c_tile_piece(const char *src, char *lds)
+{
+    __builtin_amdgcn_global_load_lds((p2c_glb_ptr)src, (p2c_lds_ptr)lds, 16, 0, 0);
 }
 
 // Waits until at most N of this wave's copies are in flight and every LDS read it issued has returned, then meets the workgroup.

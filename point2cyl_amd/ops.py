@@ -1630,12 +1630,23 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
 
 # ------------------------------------------------------------------------------------------ 8-bit linear layers (csrc/int8.hip)
 class Int8Rows:
-    """Rows in 8 bits: `q` (M, K) int8 and `scale` (M,) fp32, x ~ q * scale[:, None].  `q` is a view of rows padded to a multiple of 64 bytes with
-    zeros (what the products read)."""
+    """Rows in 8 bits: `q` (M, K) int8 and `scale` (M,) fp32, x ~ q * scale[:, None].  `q` is a view of `store`, whose rows are padded to a multiple of 64
+    bytes with zeros (what the products read)."""
     __slots__ = ("store", "scale", "K")
 
     def __init__(self, store, scale, K):
+        _lib.require_device(store, scale)
+        if store.dtype != torch.int8 or store.dim() != 2 or store.shape[1] != (K + 63) // 64 * 64 or not store.is_contiguous() or store.data_ptr() % 16 or K < 1:
+            raise ValueError("Int8Rows: the rows are contiguous int8 (M, %d) for K = %d, got %s %s" % ((K + 63) // 64 * 64, K, store.dtype, tuple(store.shape)))
+        if scale.dtype != torch.float32 or tuple(scale.shape) != store.shape[:1] or not scale.is_contiguous() or scale.device != store.device:
+            raise ValueError("Int8Rows: one fp32 scale per row on the rows' device, got %s %s on %s" % (scale.dtype, tuple(scale.shape), scale.device))
         self.store, self.scale, self.K = store, scale, K
+
+    @classmethod
+    def _of(cls, store, scale, K):                 # (tensors made here need no checks)
+        rows = cls.__new__(cls)
+        rows.store, rows.scale, rows.K = store, scale, K
+        return rows
 
     @property
     def q(self):
@@ -1684,7 +1695,7 @@ def quantize_rows(x):
     with _lib.on(x.device):
         call("p2c_quantize_rows", ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K, M, K, Kp, ptr(q), ptr(scale), stream(),
              nbytes=float(M) * (K * x.element_size() + Kp))
-    return Int8Rows(q, scale, K)
+    return Int8Rows._of(q, scale, K)
 
 
 class Int8Weight:
@@ -1768,7 +1779,7 @@ def linear_int8(x, w, act="none", beta=100.0, threshold=20.0, add=None, out_dtyp
             q = torch.empty(M, ldo, dtype=torch.int8, device=dev)
             so = torch.empty(M, dtype=torch.float32, device=dev)
             call("p2c_int8_linear_requant", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(q), ldo, ptr(so), M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
-            return Int8Rows(q, so, w.N)
+            return Int8Rows._of(q, so, w.N)
         out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
         if M == 0:
             pass

@@ -95,16 +95,14 @@ class Muon(Adam):
     number (chunks of 24), momentum, norm, normalisation, decay and update included.  Vectors and scalars (biases, BatchNorm), and every parameter of a
     group with use_muon=False, take Adam's rule with the group's `betas` and `adam_eps` in one launch, without decay.
 
-    fp32, contiguous; `param_groups`, `state_dict` keep torch's shapes (state: "momentum_buffer" for matrices, Adam's three for the others).  The
-    workspace is the optimizer's own: one optimizer steps on one stream at a time."""
+    fp32, contiguous; `param_groups`, `state_dict` keep torch's shapes (state: "momentum_buffer" for matrices, Adam's three for the others).  A step can
+    be captured into a graph after one eager step has made the state; its replays keep the learning rates (and Adam's step count) of the capture."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, ns_coeffs=ops.NS_COEFFS, eps=1e-7, adjust="rms",
                  betas=(0.9, 0.999), adam_eps=1e-8, use_muon=True):
         torch.optim.Optimizer.__init__(self, params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
                                                           ns_coeffs=ns_coeffs, eps=eps, adjust=adjust, betas=betas, adam_eps=adam_eps, use_muon=use_muon))
-        self._tables, self._mats, self._ws = {}, {}, None
-        for g in self.param_groups:
-            self._check_group(g)
+        self._tables, self._mats = {}, {}
 
     @staticmethod
     def _check_group(g):
@@ -121,18 +119,19 @@ class Muon(Adam):
         self._mats = {}
 
     def add_param_group(self, param_group):
+        self._check_group({**self.defaults, **param_group})
         super().add_param_group(param_group)
         self._mats = {}
-        if hasattr(self, "_ws"):                   # (not during construction)
-            self._check_group(self.param_groups[-1])
 
     def _matrices(self, gi, ps, group):
         """Descriptors of the group's matrices, rebuilt when a pointer, the learning rate or the decay changed."""
         for p in ps:
             if "momentum_buffer" not in self.state[p]:
+                if torch.cuda.is_current_stream_capturing():       # (the zeros would be part of the graph: every replay would start the momentum again)
+                    raise RuntimeError("point2cyl_amd.optim.Muon: take one step before capturing one (a parameter has no momentum yet)")
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
         lr, wd, adjust = float(group["lr"]), float(group["weight_decay"]), group["adjust"]
-        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]), *[(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps])
+        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]), *[(p.data_ptr(), p.grad.data_ptr(), p.grad.stride(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps])
         hit = self._mats.get(gi)
         if hit is not None and hit[0] == key:
             return hit
@@ -172,10 +171,9 @@ class Muon(Adam):
                 with _lib.on(mats[0].device):
                     _, rec, n, nb, co, _ = self._matrices(gi, mats, group)
                     if n:
-                        if self._ws is None or self._ws.numel() < nb or self._ws.device != mats[0].device:
-                            self._ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=mats[0].device)
+                        ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=mats[0].device)        # (of this call: a captured step keeps its own)
                         call("p2c_muon_step_f32", rec, n, float(group["momentum"]), int(bool(group["nesterov"])), int(group["ns_steps"]), co,
-                             float(group["eps"]), ptr(self._ws), self._ws.numel(), stream())
+                             float(group["eps"]), ptr(ws), ws.numel(), stream())
             if rest:
                 self._adam(gi, rest, group["lr"], group["betas"], group["adam_eps"])
         return loss

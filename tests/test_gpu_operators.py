@@ -370,6 +370,25 @@ def test_linear_int8_requantized(M, K, N, act, with_add):
     assert ((back - want).abs() <= tol + h.scale.double()[:, None] * 0.5001).all()   # half a quantum
 
 
+@pytest.mark.parametrize("M,K,N", [(65536, 128, 512), (66001, 65, 300), (98304 + 5, 200, 257), (131200, 387, 512), (66001, 64, 300)])
+@pytest.mark.parametrize("act,with_add", [("softplus", False), ("relu", True), ("none", False)])
+def test_linear_int8_requantized_many_rows(M, K, N, act, with_add):
+    """Calls of many workgroups: every row is what a call with few rows makes of it."""
+    from point2cyl_amd import ops
+    r = gen(21)
+    x, W, b = r(M, K), r(N, K) / K ** 0.5, r(N) * 0.1
+    x[M - 1, 0], x[40000, K - 1], x[777] = float("nan"), float("inf"), 0.0
+    add = r(M, N) if with_add else None
+    w, rows = ops.Int8Weight(W, b), ops.quantize_rows(x)
+    h = ops.linear_int8(rows, w, act=act, add=add, requantize=True)
+    again = ops.linear_int8(rows, w, act=act, add=add, requantize=True)
+    assert torch.equal(h.store, again.store) and same_scale(h.scale, again.scale)
+    assert torch.isnan(h.scale[[M - 1, 40000]]).all() and not h.q[[M - 1, 40000]].any() and int(torch.isnan(h.scale).sum()) == 2
+    for i in list(range(0, M, 13001)) + [M - 700]:
+        part = ops.linear_int8(x[i:i + 700], w, act=act, add=None if add is None else add[i:i + 700], requantize=True)
+        assert torch.equal(h.store[i:i + 700], part.store) and same_scale(h.scale[i:i + 700], part.scale)
+
+
 def test_linear_int8_addend_bias_and_views():
     from point2cyl_amd import ops
     r = gen(13)
@@ -437,7 +456,9 @@ def test_int8_refusals():
                  (lambda: ops.linear_int8(x, w, act="softplus", beta=0.0), ValueError), (lambda: ops.linear_int8(x, w, out_dtype=torch.float64), TypeError),
                  (lambda: ops.linear_int8(x, w, add=x), ValueError), (lambda: ops.linear_int8(x, w, requantize=True, out_dtype=torch.float32), ValueError),
                  (lambda: ops.linear_int8(x[None], w, requantize=True), ValueError), (lambda: ops.linear_int8(x.clone().requires_grad_(), w), RuntimeError),
-                 (lambda: ops.linear_int8(x.cpu(), w), RuntimeError), (lambda: ops.quantize_rows(x).dequantize(torch.int32), TypeError)):
+                 (lambda: ops.linear_int8(x.cpu(), w), RuntimeError), (lambda: ops.Int8Rows(w.q[:6, :8], w.scale[:6], 8), ValueError),
+                 (lambda: ops.Int8Rows(w.q[:6], w.scale[:5], 8), ValueError), (lambda: ops.Int8Rows(w.q[:6].float(), w.scale[:6], 8), ValueError),
+                 (lambda: ops.Int8Rows(w.q[:6], w.scale[:6], 65), ValueError), (lambda: ops.quantize_rows(x).dequantize(torch.int32), TypeError)):
         with pytest.raises(e):
             f()
 
@@ -491,6 +512,43 @@ def test_operators_on_another_stream_and_in_a_graph():
     for _ in range(4):
         o2.step()
     assert torch.equal(p, p2) and torch.equal(q, q2)
+
+
+def test_captured_steps_keep_their_workspace():
+    """Two steps captured from one optimizer, eager steps of a larger one and allocations between their replays."""
+    from point2cyl_amd import optim
+    r = gen(22)
+    base = [r(100, 200), r(2000, 8), r(130, 70)]
+    ps, qs = ([torch.nn.Parameter(t.clone()) for t in base] for _ in range(2))
+    gs = [r(*t.shape) for t in base]
+    for p, q, g in zip(ps, qs, gs):
+        p.grad, q.grad = g.clone(), g.clone()
+    o, o2 = optim.Muon(ps, lr=0.01), optim.Muon(qs, lr=0.01)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        fresh = optim.Muon([torch.nn.Parameter(r(40, 50))], lr=0.01)
+        fresh.param_groups[0]["params"][0].grad = r(40, 50)
+        with pytest.raises(RuntimeError, match="one step before"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=st):
+            fresh.step()
+        o.step()
+        graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+        for g in graphs:
+            with torch.cuda.graph(g, stream=st):
+                o.step()
+    big = torch.nn.Parameter(r(700, 900))
+    big.grad = r(700, 900)
+    other = optim.Muon([big], lr=0.01)
+    for k in range(3):
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        ps[0].grad.copy_(gs[0] * (k + 2)), other.step(), torch.full((1 << 22,), 3.0, device="cuda")
+        torch.cuda.synchronize()
+    for k in range(7):
+        qs[0].grad.copy_(gs[0] * (1 if k < 3 else (k + 1) // 2))
+        o2.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
 
 
 # ------------------------------------------------------------------------------------------ the paths that use them

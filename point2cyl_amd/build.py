@@ -60,8 +60,9 @@ def build(force=False, verbose=False):
     deps = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "fwd_pp.h"), os.path.join(CSRC, "tile_dma.h"), os.path.join(CSRC, "lsa.h"), os.path.join(CSRC, "eigh3.h"), os.path.join(HERE, "..", "include", "p2c_hip.h")]
     objs, dirty = [], False
     procs = []
-    stamp = os.path.join(OBJ, "flags.txt")                 # objects built with other options are stale whatever their age
-    if not os.path.exists(stamp) or open(stamp).read() != " ".join(FLAGS) + repr(sorted(EXTRA.items())):
+    # objects built with other options are stale whatever their age
+    stamps = {os.path.join(OBJ, "flags.txt"): " ".join(FLAGS), os.path.join(OBJ, "extra.txt"): repr(sorted(EXTRA.items()))}
+    if any(not os.path.exists(f) or open(f).read() != text for f, text in stamps.items()):
         force = True
     for src in SOURCES:
         s = os.path.join(CSRC, src)
@@ -85,8 +86,9 @@ def build(force=False, verbose=False):
         if verbose:
             print(" ".join(cmd))
         subprocess.check_call(cmd)
-        with open(stamp, "w") as f:
-            f.write(" ".join(FLAGS) + repr(sorted(EXTRA.items())))
+        for name, text in stamps.items():
+            with open(name, "w") as f:
+                f.write(text)
     return LIB
 
 

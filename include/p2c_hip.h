@@ -601,7 +601,9 @@ int p2c_muon_step_f32(const p2c_ns_matrix *mats_host, int n, float momentum, int
  *   p2c_int8_linear: out[r][n] = act((sum_k xq wq) sx[r] sw[n] + bias[n] + add[r][n]); act 0 none, 1 ReLU, 2 softplus(beta, thr); bias, add may be NULL.
  *   p2c_int8_linear_requant (N <= 512; softplus: thr >= 17): the same result as quantised rows out [M][ldo = p2c_int8_padded(N)], so [M]; the fp32
  *     values never reach memory.
- *   p2c_int8_linear_few (M <= 32, K <= 2048): x as floats of xdtype, quantised in the same launch. */
+ *   p2c_int8_linear_few (M <= 32, K <= 2048): x as floats of xdtype, quantised in the same launch.
+ *   p2c_int8_linear_float, _requant_float: x as floats, any M; ws: M * Kp + 4 M bytes, 16-byte aligned (the quantised rows; NULL where
+ *     p2c_int8_few_supported for _float). */
 int p2c_int8_padded(int K);
 int p2c_int8_padded_out(int N);
 int p2c_int8_few_supported(int M, int K);
@@ -614,6 +616,12 @@ int p2c_int8_linear_requant(const int8_t *xq, long long ldx, const float *sx, co
                             long long ldadd, int act, float beta, float thr, int8_t *out, int ldo, float *so, int M, int N, int K, int Kp, void *stream);
 int p2c_int8_linear_few(const void *x, int xdtype, long long ldx, const int8_t *wq, const float *sw, const float *bias, const float *add,
                         long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp, void *stream);
+int p2c_int8_linear_float(const void *x, int xdtype, long long ldx, const int8_t *wq, const float *sw, const float *bias, const float *add,
+                          long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp, void *ws,
+                          void *stream);
+int p2c_int8_linear_requant_float(const void *x, int xdtype, long long ldx, const int8_t *wq, const float *sw, const float *bias, const float *add,
+                                  long long ldadd, int act, float beta, float thr, int8_t *out, int ldo, float *so, int M, int N, int K, int Kp, void *ws,
+                                  void *stream);
 
 #ifdef __cplusplus
 }

@@ -127,6 +127,8 @@ _SIGS.update({
     "p2c_int8_linear": [c_p, c_ll, c_p, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p],
     "p2c_int8_linear_requant": [c_p, c_ll, c_p, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_p],
     "p2c_int8_linear_few": [c_p, c_i, c_ll, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p],
+    "p2c_int8_linear_float": [c_p, c_i, c_ll, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p, c_p],
+    "p2c_int8_linear_requant_float": [c_p, c_i, c_ll, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_p, c_p],
 })
 
 

@@ -36,6 +36,7 @@ __device__ __forceinline__ void p2c_tile_piece(const char *src, char *lds)
 template <int N>
 __device__ __forceinline__ void p2c_tile_wait()
 {
+    static_assert(N < 64, "vmcnt has six bits");
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);         // (vmcnt N, lgkmcnt 0; as a builtin, so that the compiler knows what has arrived)
     asm volatile("" ::: "memory");

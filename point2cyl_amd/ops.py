@@ -1773,20 +1773,27 @@ def linear_int8(x, w, act="none", beta=100.0, threshold=20.0, add=None, out_dtyp
     epi = (ptr(w.q), ptr(w.scale), ptr(w.bias), ptr(add), ldadd, _INT8_ACTS[act], float(beta), float(threshold))
     L = _lib.lib()
     with _lib.on(dev):
+        if rows is None:                           # the 8-bit rows of floats live in a workspace of this call
+            few = L.p2c_int8_few_supported(M, K) and not requantize
+            ws = None if few else torch.empty(M * (w.Kp + 4), dtype=torch.int8, device=dev)
+            xin = (ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K)
         if requantize and L.p2c_int8_requant_supported(w.N, _INT8_ACTS[act], float(threshold)):
-            rows = rows or quantize_rows(x)
             ldo = (w.N + 63) // 64 * 64
             q = torch.empty(M, ldo, dtype=torch.int8, device=dev)
             so = torch.empty(M, dtype=torch.float32, device=dev)
-            call("p2c_int8_linear_requant", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(q), ldo, ptr(so), M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
+            if M == 0:
+                pass
+            elif rows is None:
+                call("p2c_int8_linear_requant_float", *xin, *epi, ptr(q), ldo, ptr(so), M, w.N, K, w.Kp, ptr(ws), stream(), flops=2.0 * M * w.N * K)
+            else:
+                call("p2c_int8_linear_requant", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(q), ldo, ptr(so), M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
             return Int8Rows._of(q, so, w.N)
         out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
         if M == 0:
             pass
-        elif rows is None and L.p2c_int8_few_supported(M, K):
-            call("p2c_int8_linear_few", ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K, *epi, ptr(out), w.N, _DTYPES[out_dtype], M, w.N, K, w.Kp, stream())
+        elif rows is None:
+            call("p2c_int8_linear_float", *xin, *epi, ptr(out), w.N, _DTYPES[out_dtype], M, w.N, K, w.Kp, ptr(ws), stream(), flops=2.0 * M * w.N * K)
         else:
-            rows = rows or quantize_rows(x)
             call("p2c_int8_linear", ptr(rows.store), w.Kp, ptr(rows.scale), *epi, ptr(out), w.N, _DTYPES[out_dtype], M, w.N, K, w.Kp, stream(), flops=2.0 * M * w.N * K)
         if requantize:
             return quantize_rows(out)

@@ -514,6 +514,25 @@ def test_operators_on_another_stream_and_in_a_graph():
     assert torch.equal(p, p2) and torch.equal(q, q2)
 
 
+def test_two_streams_at_once():
+    from point2cyl_amd import ops
+    r = gen(23)
+    sets = [([r(300, 500), r(64, 200)], r(5000, 300), ops.Int8Weight(r(400, 300) / 17)), ([r(500, 300), r(90, 90)], r(9, 300), ops.Int8Weight(r(130, 300) / 17))]
+
+    def run(s):
+        return [*ops.newton_schulz(s[0]), ops.linear_int8(s[1], s[2]), ops.linear_int8(s[1], s[2], act="relu", requantize=True).dequantize()]
+    want = [run(s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(run(sets[k]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in range(2) for one in got[k] for a, b in zip(want[k], one))
+
+
 def test_captured_steps_keep_their_workspace():
     """Two steps captured from one optimizer, eager steps of a larger one and allocations between their replays."""
     from point2cyl_amd import optim

@@ -71,6 +71,17 @@ def test_int8_entries_refuse_bad_arguments():
     assert rq(M=0) == 0 and rq(N=513, ldo=576) == -1 and rq(ldo=128) == -1 and rq(so=None) == -1 and rq(out=ctypes.c_void_p(8)) == -2
     few = lambda **k: L.p2c_int8_linear_few(*[{**good, "x": ONE, "xdt": 0, "ldx": 8, **k}[n] for n in ("x", "xdt", "ldx", "wq", *names[4:])])  # noqa: E731
     assert few(M=33) == -1 and few(K=2049, Kp=2112) == -1 and few(x=None) == -1 and few(xdt=5) == -1 and few(M=0) == -1
+    flo = lambda **k: L.p2c_int8_linear_float(*[{**good, "x": ONE, "xdt": 0, "ldx": 8, "M": 40, "ws": ONE, **k}[n]  # noqa: E731
+                                                for n in ("x", "xdt", "ldx", "wq", *names[4:18], "ws", "st")])
+    assert flo(M=0) == 0 and flo(M=0, ws=None, x=None) == 0
+    for bad in (dict(x=None), dict(ws=None), dict(wq=None), dict(sw=None), dict(out=None), dict(xdt=5), dict(ldx=-1), dict(act=3), dict(act=2, beta=0.0), dict(dt=3), dict(ldo=7),
+                dict(add=ONE, ldadd=7), dict(N=0), dict(K=0), dict(Kp=100), dict(M=-1), dict(M=4, x=None), dict(M=4, K=2049, Kp=2112, ws=None)):
+        assert flo(**bad) == -1, bad
+    assert flo(wq=ctypes.c_void_p(8)) == -2 and flo(ws=ctypes.c_void_p(8)) == -2
+    rqf = lambda **k: L.p2c_int8_linear_requant_float(*[{**good, "x": ONE, "xdt": 0, "ldx": 8, "ldo": 64, "so": ONE, "ws": ONE, **k}[n]  # noqa: E731
+                                                        for n in ("x", "xdt", "ldx", "wq", *names[4:13], "so", *names[14:18], "ws", "st")])
+    assert rqf(M=0) == 0 and rqf(N=513, ldo=576) == -1 and rqf(ldo=128) == -1 and rqf(so=None) == -1 and rqf(ws=None) == -1 and rqf(x=None) == -1 and rqf(M=-1) == -1
+    assert rqf(act=2, thr=5.0) == -1 and rqf(out=ctypes.c_void_p(8)) == -2 and rqf(wq=ctypes.c_void_p(8)) == -2
 
 
 def test_coefficients():

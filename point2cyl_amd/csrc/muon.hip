@@ -1136,8 +1136,11 @@ inline int ns_starts(NsTab &a, int phase, int tile)
 template <int PH>
 int ns_product_any(const NsTab *tab, const NsRec *recs, int tile, int grid, float ca, float cb, int cur, hipStream_t st)
 {
-    if (PH <= 2 && tile == 96) return ns_product<128, 64, 1, 3, PH <= 2 ? PH : 1>(tab, recs, grid, ca, cb, cur, st);
-    if (PH >= 3 && tile == 128) return ns_product<128, 128, 1, 2, PH >= 3 ? PH : 3>(tab, recs, grid, ca, cb, cur, st);
+    if constexpr (PH <= 2) {
+        if (tile == 96) return ns_product<128, 64, 1, 3, PH>(tab, recs, grid, ca, cb, cur, st);
+    } else {
+        if (tile == 128) return ns_product<128, 128, 1, 2, PH>(tab, recs, grid, ca, cb, cur, st);
+    }
     if (tile == 64) return ns_product<64, 64, 1, 3, PH>(tab, recs, grid, ca, cb, cur, st);
     return ns_product<32, 32, 4, PH == 1 ? 3 : 2, PH>(tab, recs, grid, ca, cb, cur, st);
 }

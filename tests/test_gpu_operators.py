@@ -114,6 +114,39 @@ def test_newton_schulz_lists_batches_and_strides():
             check_ns(x, y)
 
 
+@pytest.mark.parametrize("shape,dtype", [((12, 700, 500), torch.float32), ((20, 385, 513), torch.bfloat16), ((300, 100, 90), torch.float16), ((257, 33, 40), torch.float32),
+                                         ((2, 1153, 2047), torch.float32)])
+def test_newton_schulz_large_batches(shape, dtype):
+    """Enough work for the large tiles; one matrix of the batch zero, one with a NaN."""
+    from point2cyl_amd import ops
+    G = (gen(24)(*shape) * torch.logspace(-3, 3, shape[0], device="cuda")[:, None, None]).to(dtype)
+    if shape[0] > 2:
+        G[1] = 0
+        G[2, -1, -1] = float("nan")
+    o = ops.newton_schulz(G)
+    for i in (0, shape[0] // 2, shape[0] - 1):
+        check_ns(o[i], G[i])
+    if shape[0] > 2:
+        assert not o[1].any() and torch.isnan(o[2]).all() and int(torch.isnan(o).any(-1).any(-1).sum()) == 1
+    assert torch.equal(torch.nan_to_num(o), torch.nan_to_num(ops.newton_schulz(G)))
+    if dtype == torch.float32:                        # the same matrices as transposed and strided views: the same numbers
+        wide = torch.zeros(shape[0], shape[2], 2 * shape[1], device="cuda")
+        wide[:, :, ::2] = G.transpose(1, 2)
+        for i in (0, shape[0] - 1):
+            check_ns(ops.newton_schulz(wide[:, :, ::2])[i], G[i].t())
+
+
+def test_newton_schulz_large_list_and_long_matrices():
+    from point2cyl_amd import ops
+    r = gen(25)
+    Gs = [r(2049, 1000), r(1025, 1500), r(33, 300), r(20, 700), r(129, 127) * 1e-4]
+    for o, G in zip(ops.newton_schulz(Gs), Gs):
+        check_ns(o, G)
+    for shape in ((33, 100000), (65537, 48), (4, 70000), (40000, 32)):
+        G = r(*shape)
+        check_ns(ops.newton_schulz(G), G)
+
+
 def test_newton_schulz_values():
     from point2cyl_amd import ops
     r = gen(5)
@@ -197,6 +230,22 @@ def test_muon_steps(nesterov, wd, adjust):
         assert (opt.state[p]["momentum_buffer"].double() - m).norm().item() <= 3 * 2.0 ** -22 * m.norm().item()
     torch.testing.assert_close(vec, vec_ref, rtol=1e-6, atol=1e-7)
     assert torch.equal(idle, idle_ref) and idle not in opt.state
+
+
+def test_muon_large_matrices():
+    from point2cyl_amd import optim
+    r = gen(26)
+    shapes = [(2049, 1000), (1025, 1500), (300, 33), (20, 700), (512, 1, 30)]
+    ps = [torch.nn.Parameter(r(*s) * 0.1) for s in shapes]
+    opt, ref = optim.Muon(ps, lr=0.02, momentum=0.9, weight_decay=0.1), Muon64(ps, 0.02, 0.9, True, 0.1, "rms")
+    for _ in range(2):
+        for p in ps:
+            p.grad = r(*p.shape) * 1e-3
+        opt.step()
+        ref.step([p.grad for p in ps])
+    for p, q, m, tol in zip(ps, ref.p, ref.m, ref.tol):
+        assert (p.detach().double() - q).norm().item() <= tol, p.shape
+        assert (opt.state[p]["momentum_buffer"].double() - m).norm().item() <= 3 * 2.0 ** -22 * m.norm().item()
 
 
 def test_muon_groups_state_and_refusals():

@@ -595,7 +595,7 @@ int p2c_muon_step_f32(const p2c_ns_matrix *mats_host, int n, float momentum, int
 /* ---------------------------------------------------------------------------------------------
  * Linear layers in 8-bit integers (csrc/int8.hip): rows and output channels carry one fp32 scale each.  dtype: 0 fp32, 1 bf16, 2 fp16.
  * Quantised rows are [M][Kp] int8 with Kp = p2c_int8_padded(K), zeros behind K; quantised weights are [p2c_int8_padded_out(N)][Kp] with zero rows
- * behind N (wq, 16-byte aligned), sw and bias [p2c_int8_padded_out(N)] with zeros behind N.  K <= 131072, M <= 2^30.
+ * behind N (wq, 16-byte aligned), sw and bias [p2c_int8_padded_out(N)] with zeros behind N.  K <= 131072, M <= 2^30; row strides of quantised rows <= 2^22.
  *   p2c_quantize_rows: s = max |row| * (1 / 127) in fp32, q = x / s to the nearest, ties to even, of the exact quotient.  A row with an infinity or a NaN: s = NaN,
  *     q = 0.  A row below 2^-119 throughout: s = 0, q = 0.  ldx: row stride of x in elements (the columns are contiguous).
  *   p2c_int8_linear: out[r][n] = act((sum_k xq wq) sx[r] sw[n] + bias[n] + add[r][n]); act 0 none, 1 ReLU, 2 softplus(beta, thr); bias, add may be NULL.

@@ -22,6 +22,8 @@ typedef _Float16 h16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 
+constexpr int I8_CUS = 256;              // an MI355X' compute units
+
 enum { Q_F32 = 0, Q_BF16 = 1, Q_F16 = 2 };
 
 __device__ __forceinline__ float q_get(const void *p, long long i, int dt)
@@ -218,10 +220,35 @@ struct I8Tile {
     static constexpr int NXC = BM * RB / 1024 / NW, NWC = BN * RB / 1024 / NW, LPW = NXC + NWC;       // copies per wave and k-tile: of x, of w, both
     static_assert(BM * RB % (1024 * NW) == 0 && BN * RB % (1024 * NW) == 0, "the same number of copies in every wave");
 
-    // meanwhile(): what is done while the first operands are on their way
-    template <class F>
-    static __device__ __forceinline__ void run(const int8_t *x, long long ldx, int lastx, const int8_t *w, long long ldw, int lastw, int KT, char *smem,
-                                               int wave, int lane, i32x16 (&acc)[TN][TM], F meanwhile)
+    // A copy's source is a scalar base plus a lane's 32-bit offset.  x: rows behind `last` are read from row `last` (their results are never stored).
+    struct RowsX {
+        const char *base;
+        unsigned at[NXC];
+        __device__ __forceinline__ void set(const int8_t *x, long long ld, int last, int wave, int lane)
+        {
+            base = (const char *)x;
+#pragma unroll
+            for (int i = 0; i < NXC; ++i) at[i] = p2c_tile_source<RB>(wave + i * NW, (int)ld, last, lane);
+        }
+    };
+    // w: never short of a row, and a piece's 16 rows repeat the swizzle, so its pieces differ by a scalar
+    struct RowsW {
+        const char *base;
+        unsigned at;
+        long long step;
+        __device__ __forceinline__ void set(const int8_t *w, int ld, int wave, int lane)
+        {
+            base = (const char *)w + (long long)wave * 16 * ld;
+            at = p2c_tile_source<RB>(0, ld, 15, lane);
+            step = (long long)NW * 16 * ld;
+        }
+    };
+
+    // One tile's sums.  FLOW: a tile follows this one with sources (xn, wn), and what is copied past this tile's end are its first k-tiles: only the `first`
+    // tile of a workgroup waits for memory.  KT >= NST then.  Without FLOW the stages are free afterwards.  now: the stage to begin with.
+    // meanwhile(): done while the very first operands are on their way.
+    template <bool FLOW, class F>
+    static __device__ __forceinline__ void run(const RowsX &sx, const RowsW &sw, const RowsX &xn, const RowsW &wn, int KT, bool first, int &now, char *smem, int wave, int lane, i32x16 (&acc)[TN][TM], F meanwhile)
     {
         const int il = lane & 31, h = lane >> 5;
 #pragma unroll
@@ -230,22 +257,21 @@ struct I8Tile {
             for (int q = 0; q < TM; ++q)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[p][q][r] = 0;
-        const char *sx[NXC], *sw[NWC];               // this lane's source of each of the wave's copies
-#pragma unroll
-        for (int i = 0; i < NXC; ++i) sx[i] = (const char *)x + p2c_tile_source<RB>(wave + i * NW, ldx, lastx, lane);
-#pragma unroll
-        for (int i = 0; i < NWC; ++i) sw[i] = (const char *)w + p2c_tile_source<RB>(wave + i * NW, ldw, lastw, lane);
-        auto copy = [&](int kt, int stage, int i) {  // (past the end: the last k-tile again, into a stage that is not multiplied: the count in flight stays exact)
-            const long long k = (long long)min(kt, KT - 1) * RB;
+        auto copy = [&](int kt, int stage, int i) {  // (nothing follows: the last k-tile again, into a stage that is not multiplied: the count in flight stays exact)
+            const bool past = FLOW && kt >= KT;
+            const long long k = (long long)(past ? kt - KT : min(kt, KT - 1)) * RB;
             char *st = smem + stage * STAGE + wave * 1024;
-            if (i < NXC) p2c_tile_piece(sx[i] + k, st + i * NW * 1024);
-            else p2c_tile_piece(sw[i - NXC] + k, st + BM * RB + (i - NXC) * NW * 1024);
+            if (i < NXC) p2c_tile_piece((past ? xn.base : sx.base) + k + (past ? xn.at[i] : sx.at[i]), st + i * NW * 1024);
+            else p2c_tile_piece((past ? wn.base : sw.base) + k + (i - NXC) * sw.step + sw.at, st + BM * RB + (i - NXC) * NW * 1024);
         };
+        if (first) {
 #pragma unroll
-        for (int s = 0; s < NST; ++s)
+            for (int s = 0; s < NST; ++s)
 #pragma unroll
-            for (int i = 0; i < LPW; ++i) copy(s, s, i);
-        meanwhile();
+                for (int i = 0; i < LPW; ++i) copy(s, s, i);
+            meanwhile();
+            p2c_tile_wait<(NST - 1) * LPW>();
+        }
         const int wr = wave / WC * (BM / WR), wc = wave % WC * (BN / WC);
         struct Frags { i32x4 x[TM], w[TN]; };
         constexpr int R = TM + TN, M = TM * TN;
@@ -270,31 +296,32 @@ struct I8Tile {
                 }
         };
         Frags f0, f1;
-        int now = 0;
-        p2c_tile_wait<(NST - 1) * LPW>();
 #pragma unroll
-        for (int i = 0; i < R; ++i) read(f0, 0, 0, i);
+        for (int i = 0; i < R; ++i) read(f0, now, 0, i);
         for (int kt = 0; kt < KT; ++kt) {
             const int next = now + 1 == NST ? 0 : now + 1;
             __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);              // f0 has arrived (lgkmcnt 0): known before the next reads are issued, or the products would wait for those
             multiply(f0, f1, now, 1, [](int) {});
-            p2c_tile_wait<(NST - 2) * LPW>();                               // k-tile kt + 1 is here; everybody has read kt
+            // k-tile kt + 1 is here; everybody has read kt.  (At the start of a following tile the last one's stores are among what is in flight: they may
+            // end out of turn, so the wait is for everything.)
+            if (FLOW && !first && kt == 0) p2c_tile_wait<0>();
+            else p2c_tile_wait<(NST - 2) * LPW>();
             multiply(f1, f0, next, 0, [&](int n) {
 #pragma unroll
                 for (int i = n * LPW / M; i < (n + 1) * LPW / M; ++i) copy(kt + NST, now, i);
             });
             now = next;
         }
-        p2c_tile_wait<0>();
+        if (!FLOW) p2c_tile_wait<0>();
     }
 };
 
-// Scales and biases of BN channels (they are padded that far; `behind`: bias of channels that do not exist) and scales of BM rows, for the LDS behind
-// the operand stages.  load() before the operands' copies, put() after: a load behind them could only be waited for with all of them.
-template <int BM, int BN, int NT>
+// Scales and biases of BN channels (they are padded that far; `behind`: bias of channels that do not exist) for the LDS.  load() before the operands'
+// copies, put() after: a load behind them could only be waited for with all of them.
+template <int BN, int NT>
 struct I8Factors {
-    float sw[(BN + NT - 1) / NT], bi[(BN + NT - 1) / NT], sx;
-    __device__ __forceinline__ void load(const I8Epi &e, int m0, int n0, int M, int N, int tid, float behind)
+    float sw[(BN + NT - 1) / NT], bi[(BN + NT - 1) / NT];
+    __device__ __forceinline__ void load(const I8Epi &e, int n0, int N, int tid, float behind)
     {
 #pragma unroll
         for (int c = 0; c < BN; c += NT)
@@ -302,7 +329,6 @@ struct I8Factors {
                 sw[c / NT] = e.sw[n0 + c + tid];
                 bi[c / NT] = n0 + c + tid >= N ? behind : e.bias ? e.bias[n0 + c + tid] : 0.f;
             }
-        if (BM >= NT || tid < BM) sx = e.sx[min(m0 + tid, M - 1)];
     }
     __device__ __forceinline__ void put(float *f, int tid, float unit) const
     {
@@ -312,7 +338,6 @@ struct I8Factors {
                 f[c + tid] = sw[c / NT] * unit;
                 f[BN + c + tid] = bi[c / NT] * unit;
             }
-        if (BM >= NT || tid < BM) f[2 * BN + tid] = sx;
     }
 };
 
@@ -331,33 +356,67 @@ __device__ __forceinline__ void i8_store8(uint16_t *row, int c, int N, u16x8 v)
         if (c + k < N) row[c + k] = v[k];
 }
 
-template <int BM, int BN, int WR, int WC, int NST, int ACT>
+// LDS: operand stages; 32 rows of a wave's result in fp32, PC pieces of 32 channels wide (with FLOW one, behind the stages, which are being filled for
+// the next tile); factors
+template <int WAVES, int BN, int TN, int OPS, bool FLOW>
+struct I8Linear {
+    static constexpr int PC = FLOW ? 1 : TN, LDF = PC * 128 + 16, PIECE = 32 * LDF, OUT = WAVES * PIECE, STAGE = FLOW ? OPS : 0;
+    static constexpr int FACT = FLOW ? OPS + OUT : OPS > OUT ? OPS : OUT, LDS = FACT + 2 * BN * 4;
+};
+
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW, int ACT>
 __global__ void __launch_bounds__(64 * WR * WC, 2) int8_linear_kernel(const int8_t *__restrict__ x, const int8_t *__restrict__ w, long long ldx, int Kp,
                                                                       int M, int N, int nbn, I8Epi e)
 {
     typedef I8Tile<BM, BN, WR, WC, NST> T;
-    constexpr int OUT = WR * WC * 32 * (T::TN * 128 + 16), OPS = NST * T::STAGE, FACT = OPS > OUT ? OPS : OUT;
-    static_assert(BM <= 64 * WR * WC, "");
+    typedef I8Linear<WR * WC, BN, T::TN, NST * T::STAGE, FLOW> L;
+    static_assert(T::TN <= 2, "32 rows in 16 bits fit where one piece in 32 does");
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), il = lane & 31, h = lane >> 5;
-    const int bm = blockIdx.x / nbn, bn = blockIdx.x - bm * nbn, m0 = bm * BM, n0 = bn * BN;
-    float *fact = reinterpret_cast<float *>(smem + FACT);
-    i32x16 acc[T::TN][T::TM];
-    I8Factors<BM, BN, 64 * WR * WC> fa;
-    fa.load(e, m0, n0, M, N, tid, 0.f);
-    T::run(x + (long long)m0 * ldx, ldx, M - 1 - m0, w + (long long)n0 * Kp, Kp, BN - 1, Kp / 64, smem, wave, lane, acc,
-           [&]() { fa.put(fact, tid, 1.0f); });
-
-    // epilogue, 32 rows x 32 TN channels of a wave at a time: finished in the registers (a lane: one row, 4 consecutive channels), through LDS in the
-    // output's type, out in 16-byte pieces along the rows.  What differs between calls is decided per piece, not per element.
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wr = wave / WC * (BM / WR), wc = wave % WC * (BN / WC);
+    float *fact = reinterpret_cast<float *>(smem + L::FACT);
+    char *stage = smem + L::STAGE + wave * L::PIECE;
     const float inv_beta = ACT == 2 ? 1.0f / e.beta : 0.f;
-    const int wr = wave / WC * (BM / WR), wc = wave % WC * (BN / WC), c0 = n0 + wc;
-    constexpr int LDF = T::TN * 128 + 16, LDB = T::TN * 64 + 16;             // bytes of a staged row, 32- and 16-bit outputs
-    char *stage = smem + wave * (32 * LDF);
+    const int tiles = (M + BM - 1) / BM * nbn;
+    typename T::RowsX xs, xn;
+    typename T::RowsW ws, wn;
+    int now = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    int tid = threadIdx.x;
+    if (FLOW) asm volatile("" : "+v"(tid));                                  // (the addresses made of it are made again for every tile: kept, they cost registers)
+    const int lane = tid & 63, il = lane & 31, h = lane >> 5;
+    const int bm = tile / nbn, bn = tile - bm * nbn, m0 = bm * BM, n0 = bn * BN, c0 = n0 + wc;
+    const bool first = !FLOW || tile == (int)blockIdx.x;
+    if (first) {
+        xs.set(x + (long long)m0 * ldx, ldx, M - 1 - m0, wave, lane);
+        ws.set(w + (long long)n0 * Kp, Kp, wave, lane);
+    }
+    if (FLOW) {
+        const int t1 = tile + (int)gridDim.x < tiles ? tile + (int)gridDim.x : tile, bm1 = t1 / nbn;          // (behind the last tile: itself once more)
+        xn.set(x + (long long)bm1 * BM * ldx, ldx, M - 1 - bm1 * BM, wave, lane);
+        wn.set(w + (long long)(t1 - bm1 * nbn) * BN * Kp, Kp, wave, lane);
+    } else {
+        xn = xs;
+        wn = ws;
+    }
+    float sx[T::TM];
+#pragma unroll
+    for (int q = 0; q < T::TM; ++q) sx[q] = e.sx[min(m0 + wr + q * 32 + il, M - 1)];
+    I8Factors<BN, 64 * WR * WC> fa;
+    fa.load(e, n0, N, tid, 0.f);
+    i32x16 acc[T::TN][T::TM];
+    T::template run<FLOW>(xs, ws, xn, wn, Kp / 64, first, now, smem, wave, lane, acc, [&]() { if (!FLOW) fa.put(fact, tid, 1.0f); });
+    if (FLOW) {
+        fa.put(fact, tid, 1.0f);                                             // (everybody is through with the last tile's)
+        __syncthreads();
+    }
+
+    // epilogue, 32 rows of a wave at a time: finished in the registers (a lane: one row, 4 consecutive channels), through LDS in the output's type, out in
+    // 16-byte pieces along the rows.  What differs between calls is decided per piece, not per element.
+    constexpr int PC = L::PC, LDF = L::LDF, LDB = T::TN * 64 + 16;           // bytes of a staged row, 32- and 16-bit outputs
 #pragma unroll
     for (int q = 0; q < T::TM; ++q) {
         const int r0 = m0 + wr + q * 32;
-        const float sx = fact[2 * BN + wr + q * 32 + il];
 #pragma unroll
         for (int p = 0; p < T::TN; ++p) {
             f32x4 v[4];
@@ -366,7 +425,7 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_linear_kernel(const int8
                 const int c = wc + p * 32 + 8 * g + 4 * h;
                 const f32x4 sw = *reinterpret_cast<const f32x4 *>(fact + c), bi = *reinterpret_cast<const f32x4 *>(fact + BN + c);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[g][k] = __builtin_fmaf((float)acc[p][q][4 * g + k] * sx, sw[k], bi[k]);
+                for (int k = 0; k < 4; ++k) v[g][k] = __builtin_fmaf((float)acc[p][q][4 * g + k] * sx[q], sw[k], bi[k]);
             }
             if (e.add) {
 #pragma unroll
@@ -381,7 +440,17 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_linear_kernel(const int8
                 }
             if (e.dtype == Q_F32) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4 *>(stage + il * LDF + (p * 32 + 8 * g + 4 * h) * 4) = v[g];
+                for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4 *>(stage + il * LDF + (p % PC * 32 + 8 * g + 4 * h) * 4) = v[g];
+                if (p % PC == PC - 1) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+                    for (int t = 0; t < 4 * PC; ++t) {                       // (stores need no more than an element's alignment)
+                        const int u = lane + 64 * t, r = u / (8 * PC), c4 = u % (8 * PC) * 4;
+                        if (r0 + r < M)
+                            i8_store4(reinterpret_cast<float *>(e.out) + (long long)(r0 + r) * e.ldo, c0 + (p - PC + 1) * 32 + c4, N, *reinterpret_cast<const f32x4 *>(stage + r * LDF + c4 * 4));
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
             } else if (e.dtype == Q_BF16) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) *reinterpret_cast<bf16x4 *>(stage + il * LDB + (p * 32 + 8 * g + 4 * h) * 2) = __builtin_convertvector(v[g], bf16x4);
@@ -390,57 +459,76 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_linear_kernel(const int8
                 for (int g = 0; g < 4; ++g) *reinterpret_cast<h16x4 *>(stage + il * LDB + (p * 32 + 8 * g + 4 * h) * 2) = __builtin_convertvector(v[g], h16x4);
             }
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (e.dtype == Q_F32) {                                              // (stores need no more than an element's alignment)
-#pragma unroll
-            for (int t = 0; t < 4 * T::TN; ++t) {
-                const int u = lane + 64 * t, r = u / (8 * T::TN), c4 = u % (8 * T::TN) * 4;
-                if (r0 + r < M) i8_store4(reinterpret_cast<float *>(e.out) + (long long)(r0 + r) * e.ldo, c0 + c4, N, *reinterpret_cast<const f32x4 *>(stage + r * LDF + c4 * 4));
-            }
-        } else {
+        if (e.dtype != Q_F32) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
             for (int t = 0; t < 2 * T::TN; ++t) {
                 const int u = lane + 64 * t, r = u / (4 * T::TN), c8 = u % (4 * T::TN) * 8;
                 if (r0 + r < M) i8_store8(reinterpret_cast<uint16_t *>(e.out) + (long long)(r0 + r) * e.ldo, c0 + c8, N, *reinterpret_cast<const u16x8 *>(stage + r * LDB + c8 * 2));
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    if (!FLOW) break;
+    xs = xn;
+    ws = wn;
+    }
+    if (FLOW) p2c_tile_wait<0>();                                            // the copies past the last tile have landed before the LDS is given back
 }
+
+// LDS of the requantising kernel: operand stages; rows of the result, maxima (with FLOW behind the stages, which are being filled for the next tile); factors
+template <int BM, int BN, int WC, int OPS, bool FLOW>
+struct I8Requant {
+    static constexpr int LDQ = BN + 16, OUT = BM * LDQ + (WC + 1) * BM * 4, QT = FLOW ? OPS : 0, TOP = QT + BM * LDQ;
+    static constexpr int FACT = FLOW ? OPS + OUT : OPS > OUT ? OPS : OUT, LDS = FACT + 2 * BN * 4;
+};
 
 // ---- the product with 8-bit rows as its result: a workgroup holds whole rows (N <= BN), so their scale is known before anything is stored and the
 // 32-bit activations never leave the registers.  out [M][ldo] int8, columns behind N zero; so [M].  Softplus is computed in units of log2(e) / beta
-// (scale and bias carry the factor, the row's scale divides it out).  Two workgroups of four waves per CU: the vector instructions of one's epilogue
-// (17 per element and an exponential) run beside the other's products.  262144 x 512 x 512 with softplus: 191 us; of its clocks 30 % go with the copies (a
-// tile of 64 rows reads all the weights: 1.2 GB through the L2s), 12 % with the activation, 10 % with the stores, 4 % with the products.  128 rows in
-// eight waves halve the copies but have no second workgroup beside them (194 us; 186 with the next tile's operands on their way during the epilogue).
-template <int BM, int BN, int WR, int WC, int NST, int ACT>
+// (scale and bias carry the factor, the row's scale divides it out).  64 rows in four waves, two workgroups per CU; with many rows 128 in eight waves, one
+// workgroup per CU that goes from tile to tile (FLOW): the next tile's operands arrive during the epilogue, and the weights are read half as often.
+// 262144 x 512 x 512 with softplus: 191 us and 180.  Of the 191's clocks 30 % went with the copies (a tile of 64 rows reads all the weights: 1.2 GB through
+// the L2s), 12 % with the activation (17 vector instructions per element and an exponential in the whole epilogue), 10 % with the stores, 4 % with the products.
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW, int ACT>
 __global__ void __launch_bounds__(64 * WR * WC, 2) int8_requant_kernel(const int8_t *__restrict__ x, const int8_t *__restrict__ w, long long ldx, int Kp,
                                                                        int M, int N, I8Epi e)
 {
     typedef I8Tile<BM, BN, WR, WC, NST> T;
-    constexpr int LDQ = BN + 16, OUT = BM * LDQ + (WC + 1) * BM * 4, OPS = NST * T::STAGE, FACT = OPS > OUT ? OPS : OUT;
+    typedef I8Requant<BM, BN, WC, NST * T::STAGE, FLOW> L;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), il = lane & 31, h = lane >> 5;
-    const int m0 = blockIdx.x * BM;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const float unit = ACT == 2 ? e.beta * 1.44269504f : 1.0f;
-    float *fact = reinterpret_cast<float *>(smem + FACT);
-    i32x16 acc[T::TN][T::TM];
-    I8Factors<BM, BN, 64 * WR * WC> fa;
-    fa.load(e, m0, 0, M, N, tid, ACT == 2 ? -__builtin_inff() : 0.f);
-    T::run(x + (long long)m0 * ldx, ldx, M - 1 - m0, w, Kp, BN - 1, Kp / 64, smem, wave, lane, acc, [&]() { fa.put(fact, tid, unit); });
-
-    int8_t *qt = reinterpret_cast<int8_t *>(smem);                           // [BM][LDQ]
-    float *rowtop = reinterpret_cast<float *>(smem + BM * LDQ);              // [WC][BM]
+    float *fact = reinterpret_cast<float *>(smem + L::FACT);
+    int8_t *qt = reinterpret_cast<int8_t *>(smem + L::QT);                   // [BM][LDQ]
+    float *rowtop = reinterpret_cast<float *>(smem + L::TOP);                // [WC][BM]
     uint32_t *live = reinterpret_cast<uint32_t *>(rowtop + WC * BM);         // [BM]: all ones, or zero for a row without a finite, normal scale
+    constexpr int LDQ = L::LDQ;
     const int wr = wave / WC * (BM / WR), wc = wave % WC * (BN / WC);
-    const I8Poly poly;
+    typename T::RowsX xs, xn;
+    typename T::RowsW ws;
+    const int tiles = (M + BM - 1) / BM;
+    int now = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));                                            // (the addresses made of it are made again for every tile: kept, they cost 40 registers)
+    const int lane = tid & 63, il = lane & 31, h = lane >> 5, m0 = tile * BM;
+    ws.set(w, Kp, wave, lane);
+    const bool first = !FLOW || tile == (int)blockIdx.x;
+    if (first) xs.set(x + (long long)m0 * ldx, ldx, M - 1 - m0, wave, lane);
+    const int m1 = tile + (int)gridDim.x < tiles ? m0 + (int)gridDim.x * BM : m0;              // (behind the last tile: itself once more)
+    if (FLOW) xn.set(x + (long long)m1 * ldx, ldx, M - 1 - m1, wave, lane);
+    else xn = xs;
     float top[T::TM], sx[T::TM];
 #pragma unroll
     for (int q = 0; q < T::TM; ++q) {
         top[q] = 0.f;
-        sx[q] = fact[2 * BN + wr + q * 32 + il];
+        sx[q] = e.sx[min(m0 + wr + q * 32 + il, M - 1)];
     }
+    I8Factors<BN, 64 * WR * WC> fa;
+    if (first) fa.load(e, 0, N, tid, ACT == 2 ? -__builtin_inff() : 0.f);
+    i32x16 acc[T::TN][T::TM];
+    T::template run<FLOW>(xs, ws, xn, ws, Kp / 64, first, now, smem, wave, lane, acc, [&]() { fa.put(fact, tid, unit); });
+    const I8Poly poly;
     // (softplus of the channels behind N: log2(1 + 2^-inf) = 0)
 #pragma unroll
     for (int p = 0; p < T::TN; ++p) {
@@ -514,6 +602,10 @@ __global__ void __launch_bounds__(64 * WR * WC, 2) int8_requant_kernel(const int
         if (m0 + r < M)
             *reinterpret_cast<u32x4 *>(reinterpret_cast<int8_t *>(e.out) + (long long)(m0 + r) * e.ldo + c) = *reinterpret_cast<const u32x4 *>(qt + r * LDQ + c) & live[r];
     }
+    if (!FLOW) break;
+    xs = xn;
+    }
+    if (FLOW) p2c_tile_wait<0>();                                            // the copies past the last tile have landed before the LDS is given back
 }
 
 // ---- few rows (M <= 32), rows as floats: one launch.  A workgroup owns 32 output channels; it quantises all rows into LDS (they are few and short)
@@ -606,49 +698,51 @@ int quantize_launch(const void *x, long long ldx, int M, int K, int Kp, int8_t *
     return P2C_OK;
 }
 
-template <int BM, int BN, int WR, int WC, int NST, int ACT>
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW, int ACT>
 int linear_launch(const int8_t *x, long long ldx, const int8_t *w, int Kp, int M, int N, const I8Epi &e, hipStream_t st)
 {
     typedef I8Tile<BM, BN, WR, WC, NST> T;
-    constexpr int OUT = WR * WC * 32 * (T::TN * 128 + 16), OPS = NST * T::STAGE, LDS = (OPS > OUT ? OPS : OUT) + (2 * BN + BM) * 4;
+    constexpr int LDS = I8Linear<WR * WC, BN, T::TN, NST * T::STAGE, FLOW>::LDS;
     static_assert(LDS <= 160 * 1024, "");
     if (LDS > 65536) {
-        const hipError_t rc = hipFuncSetAttribute((const void *)int8_linear_kernel<BM, BN, WR, WC, NST, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t rc = hipFuncSetAttribute((const void *)int8_linear_kernel<BM, BN, WR, WC, NST, FLOW, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (rc != hipSuccess) return (int)rc;
     }
-    const int nbn = p2c_cdiv(N, BN);
-    hipLaunchKernelGGL((int8_linear_kernel<BM, BN, WR, WC, NST, ACT>), dim3(p2c_cdiv(M, BM) * nbn), dim3(64 * WR * WC), LDS, st, x, w, ldx, Kp, M, N, nbn, e);
+    const int nbn = p2c_cdiv(N, BN), tiles = p2c_cdiv(M, BM) * nbn, grid = FLOW && tiles > I8_CUS ? I8_CUS : tiles;
+    hipLaunchKernelGGL((int8_linear_kernel<BM, BN, WR, WC, NST, FLOW, ACT>), dim3(grid), dim3(64 * WR * WC), LDS, st, x, w, ldx, Kp, M, N, nbn, e);
     P2C_LAUNCH_CHECK();
     return P2C_OK;
 }
-template <int BM, int BN, int WR, int WC, int NST>
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW>
 int linear_any(const int8_t *x, long long ldx, const int8_t *w, int Kp, int M, int N, const I8Epi &e, hipStream_t st)
 {
-    return e.act == 0 ? linear_launch<BM, BN, WR, WC, NST, 0>(x, ldx, w, Kp, M, N, e, st)
-         : e.act == 1 ? linear_launch<BM, BN, WR, WC, NST, 1>(x, ldx, w, Kp, M, N, e, st) : linear_launch<BM, BN, WR, WC, NST, 2>(x, ldx, w, Kp, M, N, e, st);
+    return e.act == 0 ? linear_launch<BM, BN, WR, WC, NST, FLOW, 0>(x, ldx, w, Kp, M, N, e, st)
+         : e.act == 1 ? linear_launch<BM, BN, WR, WC, NST, FLOW, 1>(x, ldx, w, Kp, M, N, e, st) : linear_launch<BM, BN, WR, WC, NST, FLOW, 2>(x, ldx, w, Kp, M, N, e, st);
 }
 
-template <int BM, int BN, int WR, int WC, int NST, int ACT>
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW, int ACT>
 int requant_launch(const int8_t *x, long long ldx, const int8_t *w, int Kp, int M, int N, const I8Epi &e, hipStream_t st)
 {
     typedef I8Tile<BM, BN, WR, WC, NST> T;
-    constexpr int OUT = BM * (BN + 16) + (WC + 1) * BM * 4, OPS = NST * T::STAGE, LDS = (OPS > OUT ? OPS : OUT) + (2 * BN + BM) * 4;
+    constexpr int LDS = I8Requant<BM, BN, WC, NST * T::STAGE, FLOW>::LDS;
     static_assert(LDS <= 160 * 1024, "");
     if (LDS > 65536) {
-        const hipError_t rc = hipFuncSetAttribute((const void *)int8_requant_kernel<BM, BN, WR, WC, NST, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t rc = hipFuncSetAttribute((const void *)int8_requant_kernel<BM, BN, WR, WC, NST, FLOW, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (rc != hipSuccess) return (int)rc;
     }
-    hipLaunchKernelGGL((int8_requant_kernel<BM, BN, WR, WC, NST, ACT>), dim3(p2c_cdiv(M, BM)), dim3(64 * WR * WC), LDS, st, x, w, ldx, Kp, M, N, e);
+    const int tiles = p2c_cdiv(M, BM), grid = FLOW && tiles > I8_CUS ? I8_CUS : tiles;
+    hipLaunchKernelGGL((int8_requant_kernel<BM, BN, WR, WC, NST, FLOW, ACT>), dim3(grid), dim3(64 * WR * WC), LDS, st, x, w, ldx, Kp, M, N, e);
     P2C_LAUNCH_CHECK();
     return P2C_OK;
 }
-template <int BM, int BN, int WR, int WC, int NST>
+template <int BM, int BN, int WR, int WC, int NST, bool FLOW>
 int requant_any(const int8_t *x, long long ldx, const int8_t *w, int Kp, int M, int N, const I8Epi &e, hipStream_t st)
 {
-    return e.act == 0 ? requant_launch<BM, BN, WR, WC, NST, 0>(x, ldx, w, Kp, M, N, e, st)
-         : e.act == 1 ? requant_launch<BM, BN, WR, WC, NST, 1>(x, ldx, w, Kp, M, N, e, st) : requant_launch<BM, BN, WR, WC, NST, 2>(x, ldx, w, Kp, M, N, e, st);
+    return e.act == 0 ? requant_launch<BM, BN, WR, WC, NST, FLOW, 0>(x, ldx, w, Kp, M, N, e, st)
+         : e.act == 1 ? requant_launch<BM, BN, WR, WC, NST, FLOW, 1>(x, ldx, w, Kp, M, N, e, st) : requant_launch<BM, BN, WR, WC, NST, FLOW, 2>(x, ldx, w, Kp, M, N, e, st);
 }
 
+constexpr long long I8_MAX_LD = 1 << 22;       // (a tile's offsets have 32 bits)
 bool i8_shape_bad(long long M, int K, int Kp) { return M < 0 || M > (1ll << 30) || K < 1 || K > 131072 || Kp < K || Kp % 64; }
 
 }  // namespace
@@ -698,7 +792,7 @@ static int i8_epilogue(I8Epi &e, const float *sx, const float *sw, const float *
 extern "C" int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx, const int8_t *wq, const float *sw, const float *bias, const float *add,
                                long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp, void *stream)
 {
-    if (i8_shape_bad(M, K, Kp) || N < 1 || N > (1 << 20) || ldx < Kp) return P2C_EINVAL;
+    if (i8_shape_bad(M, K, Kp) || N < 1 || N > (1 << 20) || ldx < Kp || ldx > I8_MAX_LD) return P2C_EINVAL;
     I8Epi e;
     const int rc = i8_epilogue(e, sx, sw, bias, add, ldadd, act, beta, thr, out, ldo, dtype, N);
     if (rc != P2C_OK) return rc;
@@ -708,16 +802,21 @@ extern "C" int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx,
     const hipStream_t st = (hipStream_t)stream;
     // 256 x 256 reads each operand half as often as 128 x 128 (16384 x 4096 x 4096: 270 us against 384; 262144 x 512 x 512: 142 against 153), but has to
     // fill most of the 256 CUs; the same limit for 128 x 128 against 64 x 64.
-    if ((long long)p2c_cdiv(M, 256) * p2c_cdiv(N, 256) >= 192) return linear_any<256, 256, 2, 4, 3>(xq, ldx, wq, Kp, M, N, e, st);
-    if ((long long)p2c_cdiv(M, 128) * p2c_cdiv(N, 128) >= 192) return linear_any<128, 128, 2, 2, 3>(xq, ldx, wq, Kp, M, N, e, st);
-    return linear_any<64, 64, 2, 2, 4>(xq, ldx, wq, Kp, M, N, e, st);
+    // 256 x 256 reads each operand half as often as 128 x 128 (16384 x 4096 x 4096: 270 us against 384; 262144 x 512 x 512: 142 against 153), but has to
+    // fill most of the 256 CUs; the same limit for 128 x 128 against 64 x 64.  From two tiles per CU on, one workgroup takes them one after the other
+    // (16384 x 4096 x 4096: 278 -> 267 us; k-tiles for all three stages needed).
+    const long long t256 = (long long)p2c_cdiv(M, 256) * p2c_cdiv(N, 256);
+    if (t256 >= 2 * I8_CUS && Kp >= 192) return linear_any<256, 256, 2, 4, 3, true>(xq, ldx, wq, Kp, M, N, e, st);
+    if (t256 >= 192) return linear_any<256, 256, 2, 4, 3, false>(xq, ldx, wq, Kp, M, N, e, st);
+    if ((long long)p2c_cdiv(M, 128) * p2c_cdiv(N, 128) >= 192) return linear_any<128, 128, 2, 2, 3, false>(xq, ldx, wq, Kp, M, N, e, st);
+    return linear_any<64, 64, 2, 2, 4, false>(xq, ldx, wq, Kp, M, N, e, st);
 }
 
 extern "C" int p2c_int8_linear_requant(const int8_t *xq, long long ldx, const float *sx, const int8_t *wq, const float *sw, const float *bias,
                                        const float *add, long long ldadd, int act, float beta, float thr, int8_t *out, int ldo, float *so, int M, int N, int K,
                                        int Kp, void *stream)
 {
-    if (i8_shape_bad(M, K, Kp) || !p2c_int8_requant_supported(N, act, thr) || ldx < Kp || ldo != (N + 63) / 64 * 64) return P2C_EINVAL;
+    if (i8_shape_bad(M, K, Kp) || !p2c_int8_requant_supported(N, act, thr) || ldx < Kp || ldx > I8_MAX_LD || ldo != (N + 63) / 64 * 64) return P2C_EINVAL;
     I8Epi e;
     const int rc = i8_epilogue(e, sx, sw, bias, add, ldadd, act, beta, thr, out, ldo, 0, N);
     if (rc != P2C_OK) return rc;
@@ -726,7 +825,10 @@ extern "C" int p2c_int8_linear_requant(const int8_t *xq, long long ldx, const fl
     if (((uintptr_t)xq & 15) || ((uintptr_t)wq & 15) || ((uintptr_t)out & 15) || ldx % 16) return P2C_EALIGN;
     e.so = so;
     const hipStream_t st = (hipStream_t)stream;
-    return N <= 256 ? requant_any<64, 256, 1, 4, 3>(xq, ldx, wq, Kp, M, N, e, st) : requant_any<64, 512, 1, 4, 2>(xq, ldx, wq, Kp, M, N, e, st);
+    if (N <= 256) return requant_any<64, 256, 1, 4, 3, false>(xq, ldx, wq, Kp, M, N, e, st);
+    // (two tiles per CU at least; k-tiles for both stages)
+    if (p2c_cdiv(M, 128) >= 2 * I8_CUS && Kp >= 128) return requant_any<128, 512, 2, 4, 2, true>(xq, ldx, wq, Kp, M, N, e, st);
+    return requant_any<64, 512, 1, 4, 2, false>(xq, ldx, wq, Kp, M, N, e, st);
 }
 
 extern "C" int p2c_int8_linear_few(const void *x, int xdtype, long long ldx, const int8_t *wq, const float *sw, const float *bias, const float *add,

@@ -21,10 +21,10 @@ __device__ __forceinline__ int p2c_tile_at(int r, int c) { return r * RB + ((c ^
 // Piece `piece` of a tile is 1 KB of it: 1024 / RB rows.  The byte that lane `lane` fetches for it, counted from row 0 at this k; rows past `last` are
 // read from row `last` (their results are never stored).
 template <int RB>
-__device__ __forceinline__ long long p2c_tile_source(int piece, long long ld, int last, int lane)
+__device__ __forceinline__ unsigned p2c_tile_source(int piece, int ld, int last, int lane)
 {
     const int r = piece * (1024 / RB) + lane / (RB / 16);
-    return (long long)min(r, last) * ld + (((lane & (RB / 16 - 1)) ^ p2c_tile_swz<RB>(r)) << 4);
+    return (unsigned)min(r, last) * (unsigned)ld + (((lane & (RB / 16 - 1)) ^ p2c_tile_swz<RB>(r)) << 4);
 }
 // one copy of one wave; lds (the piece's place) must be wave-uniform
 __device__ __forceinline__ void p2c_tile_piece(const char *src, char *lds)

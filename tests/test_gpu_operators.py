@@ -438,6 +438,25 @@ def test_linear_int8_requantized_many_rows(M, K, N, act, with_add):
         assert torch.equal(h.store[i:i + 700], part.store) and same_scale(h.scale[i:i + 700], part.scale)
 
 
+@pytest.mark.parametrize("M,K,N", [(65536, 192, 512), (66001, 387, 254), (33000, 200, 1030), (16640, 512, 2049), (140000, 129, 256), (132000, 128, 256)])
+@pytest.mark.parametrize("act,out,with_add", [("softplus", torch.bfloat16, False), ("relu", torch.float32, True), ("none", torch.float16, False)])
+def test_linear_int8_many_rows(M, K, N, act, out, with_add):
+    """Calls large enough that a workgroup goes through several tiles: every row is what a call with few rows makes of it."""
+    from point2cyl_amd import ops
+    r = gen(27)
+    x, W, b = r(M, K), r(N, K) / K ** 0.5, r(N) * 0.1
+    x[M - 1, 0], x[7000, K - 1], x[777] = float("nan"), float("inf"), 0.0
+    add = r(M, N) if with_add else None
+    w = ops.Int8Weight(W, b)
+    y = ops.linear_int8(x, w, act=act, add=add, out_dtype=out)
+    assert torch.isnan(y[[M - 1, 7000]]).all() and int(torch.isnan(y).any(1).sum()) == 2
+    y = torch.nan_to_num(y)
+    assert torch.equal(y, torch.nan_to_num(ops.linear_int8(ops.quantize_rows(x), w, act=act, add=add, out_dtype=out)))
+    for i in list(range(0, M, 6500)) + [M - 300]:
+        part = ops.linear_int8(x[i:i + 300], w, act=act, add=None if add is None else add[i:i + 300], out_dtype=out)
+        assert torch.equal(y[i:i + 300], torch.nan_to_num(part))
+
+
 def test_linear_int8_addend_bias_and_views():
     from point2cyl_amd import ops
     r = gen(13)

@@ -206,7 +206,8 @@ def ptr(t):
 
 
 def stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())       # (current_stream().cuda_stream without the Stream object: 1 us)
+    # current_stream().cuda_stream without the Stream object and the check that the device is initialised (the callers' tensors are on it): 1.2 us
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class _Here:
@@ -222,7 +223,7 @@ _HERE_ALREADY = _Here()
 
 def on(device):
     """torch.cuda.device(device), without its cost where that device is the current one."""
-    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 class _Profile:

@@ -18,7 +18,8 @@
 // 32 k, [k / 32][row][128 bytes]: what a tile needs of a block is one run of memory, and a 32 x 32 piece of a result is 4 KB of it.  Sides are padded
 // with zeros to the tile.
 // All matrices of a call go through each product together: one launch per product, whatever their number (the descriptors ride in the arguments of
-// the first launch: no copy from the host, capturable).  Matrices whose small side is <= 32 take ns_small: one workgroup each.
+// the first launch: no copy from the host, capturable).  Matrices whose small side is <= 32 take ns_small, one workgroup each, where no larger ones are there
+// to ride with.
 #include "tile_dma.h"
 #include <math.h>
 #include <string.h>
@@ -31,7 +32,7 @@ typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_MAX = 24;              // matrices per chunk: the table stays under 4 KB of kernel arguments
-constexpr int NS_SMALL = 32;            // small sides up to here take ns_small
+constexpr int NS_SMALL = 32;            // small sides up to here can take ns_small
 constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at most
 constexpr float NS_SCALE = 4096.0f, NS_INV = 1.0f / 4096.0f;
 
@@ -1058,32 +1059,41 @@ __global__ void __launch_bounds__(256) ns_first_kernel(const NsTab a, const NsCo
 }
 
 inline int ns_pad(int v, int to) { return (v + to - 1) / to * to; }
-inline bool ns_is_small(const p2c_ns_matrix &m) { return (m.rows < m.cols ? m.rows : m.cols) <= NS_SMALL; }
+inline int ns_short(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.rows : m.cols; }
+inline int ns_long(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.cols : m.rows; }
+
+// How a chunk is run.  Matrices with a small side <= 32 take ns_small (9 us up to 4, 16 for 16 x 128, 32 for 16 x 512) - unless there are larger ones whose
+// launches they can ride in: they lengthen none of their chains and leave the first launch to the norms (the 19 backbone matrices, three of them small:
+// 158 -> 148 us; an optimizer step of theirs 161 -> 148).  Batches stay: they would bring more tiles than the others have.
+struct NsPlan { bool small[NS_MAX], mid; int tile; };           // mid: every one that is not small fits ns_mid_kernel
 
 // Tile of a chunk's products: 128 keeps the matrix units busy (a wave reads 8 KB of operands for 12 instructions), 64 has four times the
 // workgroups and a shorter chain per workgroup.  The choice is made for the widest product (all tiles); the padding of the sides follows it.  The symmetric
 // products of a chunk on 128 take 128 x 64 (code 96), as they have half the tiles (8 x 1024 x 2048, 288 or 576 tiles: 81 and 48 us or 77 and 46; 2048 x 2048,
 // 4000 x 1000, ...: 93 or 72).  256 x 128 with eight waves measured the same as 128 x 128 within 2 % both ways.
-inline int ns_tile(const p2c_ns_matrix *mats, int n)
+inline NsPlan ns_plan(const p2c_ns_matrix *mats, int n)
 {
+    NsPlan p;
+    p.mid = true;
+    auto fits = [](const p2c_ns_matrix &m) { return (long long)ns_pad(m.rows, 64) * ns_pad(m.cols, 64) <= NS_MID; };
+    int longest = 0;
+    for (int i = 0; i < n; ++i)
+        if (ns_short(mats[i]) > NS_SMALL && mats[i].batch) {
+            longest = ns_long(mats[i]) > longest ? ns_long(mats[i]) : longest;
+            p.mid = p.mid && fits(mats[i]);
+        }
     long long t128 = 0;
-    for (int i = 0; i < n; ++i)
-        if (!ns_is_small(mats[i])) t128 += (long long)((mats[i].rows + 127) / 128) * ((mats[i].cols + 127) / 128) * mats[i].batch;
-    return t128 >= 256 ? 128 : 64;
-}
-
-// every matrix of the chunk that is not small fits one workgroup (together with larger ones they ride in the tiled products at no cost)
-inline bool ns_all_mid(const p2c_ns_matrix *mats, int n)
-{
-    for (int i = 0; i < n; ++i)
-        if (!ns_is_small(mats[i]) && (long long)ns_pad(mats[i].rows, 64) * ns_pad(mats[i].cols, 64) > NS_MID) return false;
-    return true;
+    for (int i = 0; i < n; ++i) {
+        p.small[i] = ns_short(mats[i]) <= NS_SMALL && !(mats[i].batch == 1 && ns_long(mats[i]) <= longest && (!p.mid || fits(mats[i])));
+        if (!p.small[i]) t128 += (long long)((mats[i].rows + 127) / 128) * ((mats[i].cols + 127) / 128) * mats[i].batch;
+    }
+    p.tile = !p.mid && t128 >= 256 ? 128 : 64;
+    return p;
 }
 
 inline size_t ns_one_ws(const p2c_ns_matrix &m, int tile)
 {
-    if (ns_is_small(m) || !m.rows || !m.cols) return 0;
-    const int s = m.rows < m.cols ? m.rows : m.cols, l = m.rows < m.cols ? m.cols : m.rows, mP = ns_pad(s, tile), nP = ns_pad(l, tile);
+    const int mP = ns_pad(ns_short(m), tile), nP = ns_pad(ns_long(m), tile);
     return NS_PARTS * 8 + 3 * ns_xbytes(mP, nP) + 2 * ns_xbytes(mP, mP);
 }
 
@@ -1148,15 +1158,16 @@ int ns_product_any(const NsTab *tab, const NsRec *recs, int tile, int grid, floa
 // the chunk's table (without ws); returns the bytes of workspace it needs
 size_t ns_table(const p2c_ns_matrix *mats, int n, NsTab &a)
 {
-    const bool mid = ns_all_mid(mats, n);
-    const int tile = mid ? 64 : ns_tile(mats, n);
+    const NsPlan plan = ns_plan(mats, n);
+    const bool mid = plan.mid;
+    const int tile = plan.tile;
     a.nbig = a.nsmall = 0;
     a.start[NS_NORM][0] = a.start[NS_TILES][0] = a.start[NS_SYM][0] = a.start[NS_ALL][0] = a.small[0] = 0;
     size_t off = 0;
     for (int small = 0; small < 2; ++small)
         for (int i = 0; i < n; ++i) {
             const p2c_ns_matrix &q = mats[i];
-            if (!q.rows || !q.cols || !q.batch || (int)ns_is_small(q) != small) continue;
+            if (!q.rows || !q.cols || !q.batch || (int)plan.small[i] != small) continue;
             NsMat &d = a.mat[a.nbig + a.nsmall];
             d.src = (const char *)q.src; d.mom = q.mom; d.dst = (char *)q.dst;
             d.src_rs = q.src_rs; d.src_cs = q.src_cs; d.src_bs = q.src_bs;
@@ -1165,7 +1176,7 @@ size_t ns_table(const p2c_ns_matrix *mats, int n, NsTab &a)
             d.m = d.tall ? q.cols : q.rows; d.n = d.tall ? q.rows : q.cols;
             d.mP = ns_pad(d.m, tile); d.nP = ns_pad(d.n, tile);
             d.batch = q.batch; d.scale = q.scale; d.decay = q.decay;
-            d.ws = off; d.ws_bs = ns_one_ws(q, tile);
+            d.ws = off; d.ws_bs = small ? 0 : ns_one_ws(q, tile);
             off += d.ws_bs * q.batch;
             if (small) {
                 a.small[a.nsmall + 1] = a.small[a.nsmall] + q.batch;

@@ -142,6 +142,11 @@ def test_newton_schulz_large_list_and_long_matrices():
     Gs = [r(2049, 1000), r(1025, 1500), r(33, 300), r(20, 700), r(129, 127) * 1e-4]
     for o, G in zip(ops.newton_schulz(Gs), Gs):
         check_ns(o, G)
+    # small ones that ride with larger ones, and small ones too long for that, beside tiled matrices and beside those of one workgroup
+    for shapes in (((5, 3000), (200, 300), (16, 100), (300, 7), (1, 1)), ((64, 64), (3, 500), (2, 100), (128, 20), (17, 129)), ((700, 30), (33, 40))):
+        Gs = [r(*s) * 10.0 ** -i for i, s in enumerate(shapes)]
+        for o, G in zip(ops.newton_schulz(Gs), Gs):
+            check_ns(o, G)
     for shape in ((33, 100000), (65537, 48), (4, 70000), (40000, 32)):
         G = r(*shape)
         check_ns(ops.newton_schulz(G), G)

@@ -18,8 +18,8 @@
 // 32 k, [k / 32][row][128 bytes]: what a tile needs of a block is one run of memory, and a 32 x 32 piece of a result is 4 KB of it.  Sides are padded
 // with zeros to the tile.
 // All matrices of a call go through each product together: one launch per product, whatever their number (the descriptors ride in the arguments of
-// the first launch: no copy from the host, capturable).  Matrices whose small side is <= 32 take ns_small, one workgroup each, where no larger ones are there
-// to ride with.
+// the first launch: no copy from the host, capturable).  Small ones (up to 16 rows) take ns_small, one workgroup each, where no larger ones are there to ride
+// with.
 #include "tile_dma.h"
 #include <math.h>
 #include <string.h>
@@ -32,7 +32,7 @@ typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_MAX = 24;              // matrices per chunk: the table stays under 4 KB of kernel arguments
-constexpr int NS_SMALL = 32;            // small sides up to here can take ns_small
+constexpr int NS_SMALL = 16;            // small sides up to here can take ns_small
 constexpr int NS_PARTS = 1024;          // partial sums of squares per matrix at most
 constexpr float NS_SCALE = 4096.0f, NS_INV = 1.0f / 4096.0f;
 
@@ -879,13 +879,14 @@ __global__ void __launch_bounds__(512) ns_mid_kernel(const NsTab a, const NsCoef
     }
 }
 
-// ---- small side <= 32: one workgroup per matrix, in the m x m space and in 64 bits.  X_k = Q_k X_0 with Q and A polynomials of A_0 = X_0 X_0^T:
+// ---- small side <= 16: one workgroup per matrix, in the m x m space and in 64 bits.  X_k = Q_k X_0 with Q and A polynomials of A_0 = X_0 X_0^T:
 // q = a + bA + cA^2, Q <- q Q, A <- q A q.  G is read twice and nothing else moves.  64 bits are what this form needs (A holds SQUARED singular
 // values and a rounding grows by a^2 per step: 2.5e5 over five); at this size they cost less than the launches of the tiled form.
-constexpr int NS_XS = 2112;                                     // floats of a chunk of X: m rows of 64 ... 2048 elements, each padded by one
+constexpr int NS_XS = 2064;                                     // floats of a chunk of X: m rows of 128 ... 512 elements, each padded by one
 
 struct NsSmallLds {
     double A[NS_SMALL][NS_SMALL + 1], Q[NS_SMALL][NS_SMALL + 1], U[NS_SMALL][NS_SMALL + 1], V[NS_SMALL][NS_SMALL + 1];
+    double part[4][256];
     float x[NS_XS];
 };
 
@@ -903,8 +904,8 @@ __device__ __forceinline__ double ns_dot(const double (*x)[NS_SMALL + 1], const 
 template <int M>
 __device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int mi, int b, NsSmallLds &l)
 {
-    constexpr int BL = M / 2, SPLIT = 256 / (BL * BL), JC = 2048 / M, LDX = JC + 1, PER = (M * M + 255) / 256;
-    static_assert(M * LDX <= NS_XS && SPLIT <= JC, "");
+    constexpr int BL = M / 2, SPLIT = 256 / (BL * BL), JC = 2048 / M, LDX = JC + 1;
+    static_assert(M <= NS_SMALL && M * LDX <= NS_XS && SPLIT <= JC, "");
     const NsMat &d = a.mat[mi];
     const int tid = threadIdx.x, m = d.m, n = d.n;
     const int blk = tid % (BL * BL), sp = tid / (BL * BL), pi = blk / BL, pj = blk % BL;
@@ -948,71 +949,46 @@ __device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int m
             g[1][1] = fma(u1, v1, g[1][1]);
         }
     }
-    if (SPLIT == 1) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) l.A[2 * pi + (p >> 1)][2 * pj + (p & 1)] = g[p >> 1][p & 1];
-        __syncthreads();
-    } else {
-        double *part = &l.U[0][0];                              // [4][256], over U
-#pragma unroll
-        for (int p = 0; p < 4; ++p) part[p * 256 + tid] = g[p >> 1][p & 1];
-        __syncthreads();
-        if (tid < M * M) {
-            const int i = tid / M, j = tid % M, p = (i & 1) * 2 + (j & 1), at = (i >> 1) * BL + (j >> 1);
-            double s = 0.0;
+    for (int p = 0; p < 4; ++p) l.part[p][tid] = g[p >> 1][p & 1];
+    __syncthreads();
+    const bool on = tid < M * M;                                // an element of the M x M matrices each
+    const int ei = tid / M, ej = tid % M;
+    if (on) {
+        const int p = (ei & 1) * 2 + (ej & 1), at = (ei >> 1) * BL + (ej >> 1);
+        double s = 0.0;
 #pragma unroll 8
-            for (int k = 0; k < SPLIT; ++k) s += part[p * 256 + k * BL * BL + at];
-            l.A[i][j] = s;
-        }
-        __syncthreads();
+        for (int k = 0; k < SPLIT; ++k) s += l.part[p][k * BL * BL + at];
+        l.A[ei][ej] = s;
     }
+    __syncthreads();
     double tr = 0.0;
 #pragma unroll
     for (int k = 0; k < M; ++k) tr += l.A[k][k];
     const double inv = 1.0 / (sqrt(tr) + a.eps);
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        const int e = tid + 256 * q, i = e / M, j = e % M;
-        if (e < M * M) {
-            l.A[i][j] *= inv * inv;
-            l.Q[i][j] = i == j ? inv : 0.0;                     // the normalisation of X_0 rides in Q
-        }
+    if (on) {
+        l.A[ei][ej] *= inv * inv;
+        l.Q[ei][ej] = ei == ej ? inv : 0.0;                     // the normalisation of X_0 rides in Q
     }
     __syncthreads();
     for (int s = 0; s < co.steps; ++s) {
         const double c0 = co.c[s][0], c1 = co.c[s][1], c2 = co.c[s][2];
-        double vq[PER], va[PER];
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int e = tid + 256 * q, i = e / M, j = e % M;
-            if (e < M * M) l.U[i][j] = c2 * ns_dot<M>(l.A, l.A, i, j) + c1 * l.A[i][j] + (i == j ? c0 : 0.0);      // q
+        double vq = 0.0, va = 0.0;
+        if (on) l.U[ei][ej] = c2 * ns_dot<M>(l.A, l.A, ei, ej) + c1 * l.A[ei][ej] + (ei == ej ? c0 : 0.0);      // q
+        __syncthreads();
+        if (on) {
+            vq = ns_dot<M>(l.U, l.Q, ei, ej);
+            va = ns_dot<M>(l.U, l.A, ei, ej);
         }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int e = tid + 256 * q, i = e / M, j = e % M;
-            if (e < M * M) {
-                vq[q] = ns_dot<M>(l.U, l.Q, i, j);
-                va[q] = ns_dot<M>(l.U, l.A, i, j);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int e = tid + 256 * q, i = e / M, j = e % M;
-            if (e < M * M) {
-                l.Q[i][j] = vq[q];
-                l.V[i][j] = va[q];
-            }
+        if (on) {
+            l.Q[ei][ej] = vq;
+            l.V[ei][ej] = va;
         }
         __syncthreads();
         if (s + 1 < co.steps) {
-#pragma unroll
-            for (int q = 0; q < PER; ++q) {
-                const int e = tid + 256 * q, i = e / M, j = e % M;
-                if (e < M * M) l.A[i][j] = ns_dot<M>(l.V, l.U, i, j);
-            }
+            if (on) l.A[ei][ej] = ns_dot<M>(l.V, l.U, ei, ej);
             __syncthreads();
         }
     }
@@ -1051,8 +1027,7 @@ __global__ void __launch_bounds__(256) ns_first_kernel(const NsTab a, const NsCo
         const int k = ns_find(a.small, a.nsmall, id), mi = a.nbig + k, b = id - a.small[k], m = a.mat[mi].m;
         if (m <= 4) ns_small<4>(a, co, mi, b, l);
         else if (m <= 8) ns_small<8>(a, co, mi, b, l);
-        else if (m <= 16) ns_small<16>(a, co, mi, b, l);
-        else ns_small<32>(a, co, mi, b, l);
+        else ns_small<16>(a, co, mi, b, l);
         return;
     }
     ns_norm(a, id - nsmall_wg, &l.A[0][0]);
@@ -1062,9 +1037,13 @@ inline int ns_pad(int v, int to) { return (v + to - 1) / to * to; }
 inline int ns_short(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.rows : m.cols; }
 inline int ns_long(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.cols : m.rows; }
 
-// How a chunk is run.  Matrices with a small side <= 32 take ns_small (9 us up to 4, 16 for 16 x 128, 32 for 16 x 512) - unless there are larger ones whose
-// launches they can ride in: they lengthen none of their chains and leave the first launch to the norms (the 19 backbone matrices, three of them small:
-// 158 -> 148 us; an optimizer step of theirs 161 -> 148).  Batches stay: they would bring more tiles than the others have.
+// ns_small takes 9 us for small sides up to 8 and 64 columns, 12 for 5 x 500, 15 for 16 x 64, 31 for 16 x 512, 97 for 12 x 2000; the other forms take 27, 62, 27, 63
+// and 82 (and on 32 rows, which ns_small could hold as well, 27 for 32 x 64 against 47, 82 for 32 x 2000 against 273).
+inline bool ns_is_small(const p2c_ns_matrix &m) { return ns_short(m) <= 8 || (ns_short(m) <= NS_SMALL && ns_long(m) <= 1024); }
+
+// How a chunk is run.  Small matrices have a launch of their own - unless there are larger ones whose launches they can ride in: they lengthen none of their
+// chains and leave the first launch to the norms (the 19 backbone matrices, three of them small: 158 -> 148 us; an optimizer step of theirs 161 -> 148).
+// Batches stay: they would bring more tiles than the others have.
 struct NsPlan { bool small[NS_MAX], mid; int tile; };           // mid: every one that is not small fits ns_mid_kernel
 
 // Tile of a chunk's products: 128 keeps the matrix units busy (a wave reads 8 KB of operands for 12 instructions), 64 has four times the
@@ -1078,13 +1057,13 @@ inline NsPlan ns_plan(const p2c_ns_matrix *mats, int n)
     auto fits = [](const p2c_ns_matrix &m) { return (long long)ns_pad(m.rows, 64) * ns_pad(m.cols, 64) <= NS_MID; };
     int longest = 0;
     for (int i = 0; i < n; ++i)
-        if (ns_short(mats[i]) > NS_SMALL && mats[i].batch) {
+        if (!ns_is_small(mats[i]) && mats[i].batch) {
             longest = ns_long(mats[i]) > longest ? ns_long(mats[i]) : longest;
             p.mid = p.mid && fits(mats[i]);
         }
     long long t128 = 0;
     for (int i = 0; i < n; ++i) {
-        p.small[i] = ns_short(mats[i]) <= NS_SMALL && !(mats[i].batch == 1 && ns_long(mats[i]) <= longest && (!p.mid || fits(mats[i])));
+        p.small[i] = ns_is_small(mats[i]) && !(mats[i].batch == 1 && ns_long(mats[i]) <= longest && (!p.mid || fits(mats[i])));
         if (!p.small[i]) t128 += (long long)((mats[i].rows + 127) / 128) * ((mats[i].cols + 127) / 128) * mats[i].batch;
     }
     p.tile = !p.mid && t128 >= 256 ? 128 : 64;

@@ -595,9 +595,10 @@ int p2c_muon_step_f32(const p2c_ns_matrix *mats_host, int n, float momentum, int
 /* ---------------------------------------------------------------------------------------------
  * Linear layers in 8-bit integers (csrc/int8.hip): rows and output channels carry one fp32 scale each.  dtype: 0 fp32, 1 bf16, 2 fp16.
  * Quantised rows are [M][Kp] int8 with Kp = p2c_int8_padded(K), zeros behind K; quantised weights are [p2c_int8_padded_out(N)][Kp] with zero rows
- * behind N (wq, 16-byte aligned), sw and bias [p2c_int8_padded_out(N)] with zeros behind N.  K <= 131072, M <= 2^30; row strides of quantised rows <= 2^22.
+ * behind N (wq, 16-byte aligned), sw and bias [p2c_int8_padded_out(N)] with zeros behind N.  K <= 131072, M <= 2^30 - 64; row strides of quantised rows <= 2^22.
  *   p2c_quantize_rows: s = max |row| * (1 / 127) in fp32, q = x / s to the nearest, ties to even, of the exact quotient.  A row with an infinity or a NaN: s = NaN,
- *     q = 0.  A row below 2^-119 throughout: s = 0, q = 0.  ldx: row stride of x in elements (the columns are contiguous).
+ *     q = 0.  A row below 2^-119 throughout: s = 0, q = 0.  ldx: row stride of x in elements (the columns are contiguous).  More than
+ *     p2c_quantize_rows_at_once(K) rows take several launches.
  *   p2c_int8_linear: out[r][n] = act((sum_k xq wq) sx[r] sw[n] + bias[n] + add[r][n]); act 0 none, 1 ReLU, 2 softplus(beta, thr); bias, add may be NULL.
  *   p2c_int8_linear_requant (N <= 512; softplus: thr >= 17): the same result as quantised rows out [M][ldo = p2c_int8_padded(N)], so [M]; the fp32
  *     values never reach memory.
@@ -608,6 +609,7 @@ int p2c_int8_padded(int K);
 int p2c_int8_padded_out(int N);
 int p2c_int8_few_supported(int M, int K);
 int p2c_int8_requant_supported(int N, int act, float thr);
+int p2c_quantize_rows_at_once(int K);
 int p2c_quantize_rows(const void *x, int dtype, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, void *stream);
 int p2c_dequantize_rows(const int8_t *q, const float *scale, int M, int K, int Kp, void *out, int dtype, void *stream);
 int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx, const int8_t *wq, const float *sw, const float *bias, const float *add,

@@ -122,6 +122,7 @@ _SIGS.update({
     "p2c_int8_padded_out": [c_i],
     "p2c_int8_few_supported": [c_i, c_i],
     "p2c_int8_requant_supported": [c_i, c_i, c_f],
+    "p2c_quantize_rows_at_once": [c_i],
     "p2c_quantize_rows": [c_p, c_i, c_ll, c_i, c_i, c_i, c_p, c_p, c_p],
     "p2c_dequantize_rows": [c_p, c_p, c_i, c_i, c_i, c_p, c_i, c_p],
     "p2c_int8_linear": [c_p, c_ll, c_p, c_p, c_p, c_p, c_p, c_ll, c_i, c_f, c_f, c_p, c_ll, c_i, c_i, c_i, c_i, c_i, c_p],

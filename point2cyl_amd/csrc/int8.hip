@@ -680,9 +680,12 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const void *__restrict__ 
     }
 }
 
+// Rows of one launch: a grid holds fewer than 2^32 threads, and a workgroup of 256 takes four rows of up to 1024 elements or one longer row.
+inline int quantize_rows_at_once(int Kp) { return Kp <= 1024 ? 1 << 25 : 1 << 23; }
+
 // A row in a wave up to 1024 elements: 262144 x 512 fp32 in 113 us = 5.9 TB/s.  Longer ones in a workgroup.
 template <int DT>
-int quantize_launch(const void *x, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, hipStream_t st)
+int quantize_once(const void *x, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, hipStream_t st)
 {
     const int grid = p2c_cdiv(M, 4);
 #define P2C_QUANT(U_, LONG_) \
@@ -695,6 +698,16 @@ int quantize_launch(const void *x, long long ldx, int M, int K, int Kp, int8_t *
     else hipLaunchKernelGGL((quantize_long_kernel<DT>), dim3(M), dim3(256), 0, st, x, ldx, K, Kp, q, scale);
 #undef P2C_QUANT
     P2C_LAUNCH_CHECK();
+    return P2C_OK;
+}
+template <int DT>
+int quantize_launch(const void *x, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, hipStream_t st)
+{
+    const long long width = DT == Q_F32 ? 4 : 2, most = quantize_rows_at_once(Kp);
+    for (long long r = 0; r < M; r += most) {
+        const int rc = quantize_once<DT>((const char *)x + r * ldx * width, ldx, (int)(M - r < most ? M - r : most), K, Kp, q + r * Kp, scale + r, st);
+        if (rc != P2C_OK) return rc;
+    }
     return P2C_OK;
 }
 
@@ -743,7 +756,8 @@ int requant_any(const int8_t *x, long long ldx, const int8_t *w, int Kp, int M, 
 }
 
 constexpr long long I8_MAX_LD = 1 << 22;       // (a tile's offsets have 32 bits)
-bool i8_shape_bad(long long M, int K, int Kp) { return M < 0 || M > (1ll << 30) || K < 1 || K > 131072 || Kp < K || Kp % 64; }
+constexpr long long I8_MAX_M = (1 << 30) - 64; // (tiles of 64 rows in workgroups of 256: a grid holds fewer than 2^32 threads)
+bool i8_shape_bad(long long M, int K, int Kp) { return M < 0 || M > I8_MAX_M || K < 1 || K > 131072 || Kp < K || Kp % 64; }
 
 }  // namespace
 
@@ -752,6 +766,8 @@ extern "C" int p2c_int8_padded_out(int N) { return N < 1 ? 0 : (N + 255) / 256 *
 extern "C" int p2c_int8_few_supported(int M, int K) { return M >= 1 && M <= 32 && K >= 1 && K <= 2048; }
 // (the epilogue's softplus has no linear region of its own: above beta x = 17 it is the identity in 32 bits anyway, so the threshold has to lie there)
 extern "C" int p2c_int8_requant_supported(int N, int act, float thr) { return N >= 1 && N <= 512 && (act != 2 || thr >= 17.0f); }
+
+extern "C" int p2c_quantize_rows_at_once(int K) { return K < 1 ? 0 : quantize_rows_at_once(p2c_int8_padded(K)); }
 
 extern "C" int p2c_quantize_rows(const void *x, int dtype, long long ldx, int M, int K, int Kp, int8_t *q, float *scale, void *stream)
 {

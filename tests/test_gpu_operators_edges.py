@@ -1,0 +1,36 @@
+"""GPU: the dense-layer operators at the ends of what they accept: very many rows, very long matrices, large batches, extreme scales, optimizers that
+are copied, shrunk or captured."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("M,K,dtype", [((1 << 26) + 5, 3, torch.float32), ((1 << 24) + 3, 1025, torch.bfloat16)])
+def test_quantize_more_rows_than_a_launch_holds(M, K, dtype):
+    """Rows overlap in memory (row i starts at element i), so that the input stays small.  Rows around the launches' borders against the definition,
+    and every row's scale."""
+    from point2cyl_amd import _lib, ops
+    most = _lib.lib().p2c_quantize_rows_at_once(K)
+    assert M > most
+    buf = torch.rand(M + K, device="cuda", dtype=torch.float32).to(dtype)
+    x = buf.as_strided((M, K), (1, 1))
+    r = ops.quantize_rows(x)
+    assert r.shape == (M, K)
+    for lo in sorted({0, most - 3, most, most // 2, *range(2 * most - 2, M - 4, most), M - 6}):
+        if not 0 <= lo <= M - 6:
+            continue
+        v = x[lo:lo + 6].float()
+        s = v.abs().amax(1) * torch.tensor(1.0 / 127.0, device="cuda")
+        assert torch.equal(r.scale[lo:lo + 6], s), lo
+        assert torch.equal(r.q[lo:lo + 6], torch.round(v.double() / s.double()[:, None]).to(torch.int8)), lo
+        assert not r.store[lo:lo + 6, K:].any()
+    assert bool((r.scale > 0).all())

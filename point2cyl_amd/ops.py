@@ -1629,6 +1629,9 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
 
 
 # ------------------------------------------------------------------------------------------ 8-bit linear layers (csrc/int8.hip)
+_INT8_ROWS, _INT8_OUT = (1 << 30) - 64, 1 << 20      # rows and output channels a call takes (csrc/int8.hip; its entries count them in 32 bits)
+
+
 class Int8Rows:
     """Rows in 8 bits: `q` (M, K) int8 and `scale` (M,) fp32, x ~ q * scale[:, None].  `q` is a view of `store`, whose rows are padded to a multiple of 64
     bytes with zeros (what the products read)."""
@@ -1638,6 +1641,8 @@ class Int8Rows:
         _lib.require_device(store, scale)
         if store.dtype != torch.int8 or store.dim() != 2 or store.shape[1] != (K + 63) // 64 * 64 or not store.is_contiguous() or store.data_ptr() % 16 or K < 1:
             raise ValueError("Int8Rows: the rows are contiguous int8 (M, %d) for K = %d, got %s %s" % ((K + 63) // 64 * 64, K, store.dtype, tuple(store.shape)))
+        if store.shape[0] > _INT8_ROWS or K > 131072:
+            raise ValueError("Int8Rows: at most %d rows of at most 131072, got %s" % (_INT8_ROWS, tuple(store.shape)))
         if scale.dtype != torch.float32 or tuple(scale.shape) != store.shape[:1] or not scale.is_contiguous() or scale.device != store.device:
             raise ValueError("Int8Rows: one fp32 scale per row on the rows' device, got %s %s on %s" % (scale.dtype, tuple(scale.shape), scale.device))
         self.store, self.scale, self.K = store, scale, K
@@ -1680,11 +1685,13 @@ def _int8_rows_in(x, what):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad() or on a detached tensor" % what)
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
         raise ValueError("%s takes rows (M, K) with K of 1 ... 131072, got %s" % (what, tuple(x.shape)))
+    if x.shape[0] > _INT8_ROWS:
+        raise ValueError("%s takes at most %d rows, got %s" % (what, _INT8_ROWS, tuple(x.shape)))
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def quantize_rows(x):
-    """Rows (M, K) of fp32, bf16 or fp16 -> Int8Rows with a scale each: scale = max |row| * (1 / 127) in fp32, q = x / scale rounded to the nearest whole
+    """Rows (M, K) of fp32, bf16 or fp16, M up to 2^30 - 64, K up to 131072 -> Int8Rows with a scale each: scale = max |row| * (1 / 127) in fp32, q = x / scale rounded to the nearest whole
     number, ties to even (of the exact quotient).  A row that holds an infinity or a NaN has scale NaN and q = 0 (its products are NaN, the
     other rows are not touched); a row whose magnitudes are all below 2^-119 is a row of zeros."""
     x = _int8_rows_in(x, "quantize_rows")
@@ -1711,8 +1718,8 @@ class Int8Weight:
             raise ValueError("Int8Weight: bias %s does not fit the weight %s" % (tuple(bias.shape), tuple(weight.shape)))
         w = _int8_rows_in(weight, "Int8Weight")
         self.N, self.K = w.shape
-        if self.N < 1:
-            raise ValueError("Int8Weight takes at least one output channel")
+        if not 1 <= self.N <= _INT8_OUT:
+            raise ValueError("Int8Weight takes 1 ... %d output channels, got %d" % (_INT8_OUT, self.N))
         dev = w.device
         self.Kp, Np = (self.K + 63) // 64 * 64, (self.N + 255) // 256 * 256
         self.q = torch.zeros(Np, self.Kp, dtype=torch.int8, device=dev)

@@ -34,3 +34,18 @@ def test_quantize_more_rows_than_a_launch_holds(M, K, dtype):
         assert torch.equal(r.q[lo:lo + 6], torch.round(v.double() / s.double()[:, None]).to(torch.int8)), lo
         assert not r.store[lo:lo + 6, K:].any()
     assert bool((r.scale > 0).all())
+
+
+def test_int8_row_counts_past_32_bits_are_refused():
+    """The entries count rows in 32 bits: 2^32 + 5 rows must not become 5.  (Views that repeat one row: nothing of that size is allocated.)"""
+    from point2cyl_amd import ops
+    one = torch.ones(1, 1, device="cuda")
+    w = ops.Int8Weight(one)
+    for M in ((1 << 32) + 5, (1 << 31) + 5, (1 << 30) - 63):
+        x = one.expand(M, 1)
+        for f in (lambda: ops.linear_int8(x, w), lambda: ops.linear_int8(x, w, requantize=True), lambda: ops.quantize_rows(x), lambda: ops.linear_int8(x.view(1, M, 1), w)):
+            with pytest.raises(ValueError, match="rows"):
+                f()
+    for N in ((1 << 20) + 1, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="channels|rows"):
+            ops.Int8Weight(one.expand(N, 1))

@@ -8,7 +8,9 @@
 // fp16 numbers, x 2^12 = hi + lo (22 - 23 bits), a product is hi hi + hi lo + lo hi in 32-bit sums on v_mfma_f32_32x32x16_f16: the error of a
 // 32-bit product at a third of the fp16 rate, 5 times the rate of the chip's 32-bit matrix instruction.  2^12 fits because every matrix of
 // the iteration is bounded by a small spectral norm (the host refuses coefficients that leave (0, 15)); what drops below the fp16 range is
-// < 2^-37 of one.
+// < 2^-37 of one.  That floor is absolute where a 32-bit number's is relative, so the steps must not bring it up: the host refuses steps that amplify
+// weak directions by more than 2^15 together (rows 1e-9 of the others, 64 x 128: 1.5e-6 off after 5 steps, 2.3e-6 after 8 = 2^14.3, plain 32-bit arithmetic 1.3e-6
+// and 1.9e-6; after 10 it would be 1.0e-5 against 2.2e-6, after 16 1.7e-2 against 2.3e-6).
 // a X is added to the finished product in 32 bits and not folded into the polynomial's diagonal: folded, the rounding of a + ... hits the weak
 // directions (3.7e-5 against 1.3e-5 on a low-rank 512 x 512 gradient; 1.1e-5 for plain 32-bit arithmetic).
 //
@@ -1227,19 +1229,26 @@ int ns_run(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, int 
     NsCoef co;
     co.steps = steps;
     // every matrix of the iteration has to stay inside the range of the scaled fp16 pairs: follow the bound of the spectrum
-    double top = 1.0;
+    double top = 1.0, gain[16];
     for (int s = 0; s < steps; ++s) {
         const double c0 = coeffs[3 * s], c1 = coeffs[3 * s + 1], c2 = coeffs[3 * s + 2];
         if (!isfinite(c0) || !isfinite(c1) || !isfinite(c2)) return P2C_EINVAL;
         double p = 0.0, q = 0.0;
+        gain[s] = 0.0;
         for (int k = 0; k <= 64; ++k) {
             const double x = top * k / 64, t = x * x, bb = c1 * t + c2 * t * t, qq = c0 + bb;
             p = fmax(p, fabs(x * qq));
             q = fmax(q, fmax(fabs(bb), fabs(c0)));
+            gain[s] = fmax(gain[s], fabs(qq));
         }
         if (!(p < 3.8) || !(q < 15.0)) return P2C_EINVAL;
         top = 1.01 * p;
         for (int k = 0; k < 3; ++k) co.c[s][k] = coeffs[3 * s + k];
+    }
+    double grown = 1.0;                                          // by the steps from s on: what the pairs drop at s
+    for (int s = steps - 1; s >= 0; --s) {
+        grown *= gain[s];
+        if (!(grown <= 32768.0)) return P2C_EINVAL;
     }
     for (int s = steps; s < 16; ++s) co.c[s][0] = co.c[s][1] = co.c[s][2] = 0.f;
     for (int i = 0; i < n; ++i) {

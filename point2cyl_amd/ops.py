@@ -1566,14 +1566,20 @@ def _ns_coefficients(steps, coeffs):
     rows = [tuple(coeffs)] * steps if not hasattr(coeffs[0], "__len__") else [tuple(c) for c in coeffs]
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError("newton_schulz: coeffs are one (a, b, c), or one for each of the %d steps" % steps)
-    top = 1.0
+    top, gains = 1.0, []
     for a, b, c in rows:                   # the same bounds as csrc/muon.hip: every matrix of the iteration has to fit a scaled fp16 pair
         x = [top * k / 256 for k in range(257)]
         p = max(abs(v * (a + b * v * v + c * v ** 4)) for v in x)
         q = max([abs(a)] + [abs(b * v * v + c * v ** 4) for v in x])
+        gains.append(max(abs(a + b * v * v + c * v ** 4) for v in x))
         if not (p < 3.8 and q < 15.0):
             raise ValueError("newton_schulz: the coefficients (%g, %g, %g) drive the iteration out of range (|X| up to %g)" % (a, b, c, p))
         top = 1.01 * p
+    gain = 1.0                             # ... and what a pair cannot hold of a weak direction must not grow to where 32 bits would have kept it
+    for g in reversed(gains):
+        gain *= g
+        if not gain <= 32768.0:
+            raise ValueError("newton_schulz: the %d steps amplify weak directions by more than 2^15 (eight steps of %g)" % (steps, NS_COEFFS[0]))
     return (ctypes.c_float * (3 * steps))(*[v for r in rows for v in r])
 
 
@@ -1591,6 +1597,9 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """The orthogonalised form of a matrix (r, c), of every matrix of a batch (..., r, c), or of every matrix of a list (any shapes, one device):
     X_0 = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T of the smaller side - all singular values are driven
     towards 1, the singular vectors stay.  fp32, bf16 or fp16, any strides; 32-bit accuracy inside whatever the type, one rounding at the end.
+    Steps that together amplify the weakest directions by more than 2^15 are refused (up to eight of the default coefficients are taken): beyond that
+    rows 1e-9 of the others, which 32-bit numbers keep, would be lost.  The path goes by the whole call,
+    so a matrix may differ in its last bits alone and in a list.
     A zero matrix gives zeros; a matrix that holds an infinity or a NaN gives NaN (others of the call are not touched).  The result is
     contiguous and has no gradient.  Reference use: an update rule beside torch.optim.Adam (train_Point2Cyl_without_sketch.py:204)."""
     many = not isinstance(G, torch.Tensor)

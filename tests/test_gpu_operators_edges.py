@@ -49,3 +49,31 @@ def test_int8_row_counts_past_32_bits_are_refused():
     for N in ((1 << 20) + 1, (1 << 32) + 5):
         with pytest.raises(ValueError, match="channels|rows"):
             ops.Int8Weight(one.expand(N, 1))
+
+
+NSC = (3.4445, -4.7750, 2.0315)
+
+
+@pytest.mark.parametrize("shape", [(64, 128), (200, 60), (256, 1024), (12, 300)])
+@pytest.mark.parametrize("kind", ["half", "fall8", "fall12"])
+def test_newton_schulz_weak_rows_after_eight_steps(shape, kind):
+    """Rows far below the others, brought up by the most steps that are accepted.  An operand's absolute floor of 2^-38 enters X through A, B (|b| + 2 |c| |A| + 1 <= 12.6 of
+    them) and X itself: at most sqrt(m) 12.6 2^-38 |X| in a row's norm, m 12.6 2^-38 x 1.26 in the Frobenius norm, amplified by the steps that follow (sum of 3.4445^k).  Beside it
+    the roundings of 32-bit arithmetic: four times what the plain 32-bit form makes of the same matrix."""
+    from point2cyl_amd import ops
+    m, n = shape
+    f = {"half": torch.where(torch.arange(m) % 2 == 0, 1.0, 1e-9), "fall8": torch.logspace(0, -8, m), "fall12": torch.logspace(0, -12, m)}[kind].cuda()
+    G = gen(31)(m, n) * f[:, None]
+
+    def plain(dtype):
+        X = (G.double() / (G.double().norm() + 1e-7)).to(dtype)
+        X = X.t().contiguous() if m > n else X
+        for _ in range(8):
+            A = X @ X.t().contiguous()
+            X = NSC[0] * X + (NSC[1] * A + NSC[2] * (A @ A)) @ X
+        return X.t() if m > n else X
+    want = plain(torch.float64)
+    err = lambda o: (o.double() - want).norm().item()  # noqa: E731
+    floor = min(m, n) * 12.6 * 1.26 * 2.0 ** -38 * sum(NSC[0] ** k for k in range(8))
+    assert err(ops.newton_schulz(G, steps=8)) <= 4.0 * err(plain(torch.float32)) + floor
+    assert floor <= 4e-5 * want.norm().item()

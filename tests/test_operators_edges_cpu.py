@@ -23,3 +23,22 @@ def test_quantize_launches_fit_a_grid():
     for M in (top + 1, (1 << 31) - 1):
         assert L.p2c_quantize_rows(ONE, 0, 8, M, 8, 64, ONE, ONE, None) == -1
         assert L.p2c_int8_linear_requant(ONE, 64, ONE, ONE, ONE, None, None, 0, 0, 1.0, 20.0, ONE, 64, ONE, M, 8, 8, 64, None) == -1
+
+
+def test_newton_schulz_refuses_steps_that_amplify_too_much():
+    """The operands' floor of 2^-37 may grow to 2^-22 of one, not further: by the steps from any one to the last."""
+    L = _lib.lib()
+    a = (ctypes.c_float * 48)
+    need = 1 << 40
+    m = (_lib.NsMatrix * 1)()
+    m[0].rows, m[0].cols, m[0].batch, m[0].src, m[0].dst, m[0].src_rs, m[0].src_cs, m[0].dst_rs, m[0].dst_cs = 0, 4, 1, 16, 16, 4, 1, 4, 1       # no rows: nothing is launched
+    entry = lambda steps, co: L.p2c_newton_schulz(m, 1, 0, steps, a(*[v for c in co for v in c]), 1e-7, ONE, need, None)  # noqa: E731
+    weak, flat, strong = (1.875, -1.25, 0.375), (1.0, 0.0, 0.0), ops.NS_COEFFS
+    for co in ([strong] * 8, [weak] * 16, [strong] * 5 + [weak] * 4, [flat] * 8 + [strong] * 8, [(0.1, 0.0, 0.0)] * 4 + [strong] * 8):
+        assert len(ops.ns_coefficients(len(co), co)) == 3 * len(co) and entry(len(co), co) == 0, co
+    for co in ([strong] * 9, [strong] * 16, [strong] * 8 + [weak] * 2, [(0.1, 0.0, 0.0)] * 4 + [strong] * 9):
+        with pytest.raises(ValueError, match="2\\^15"):
+            ops.ns_coefficients(len(co), co)
+        assert entry(len(co), co) == -1, co
+    with pytest.raises(ValueError, match="2\\^15"):
+        optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], ns_steps=16)

@@ -22,9 +22,9 @@ class Adam(torch.optim.Optimizer):
         self._tables = {}
 
     def _table(self, gi, ps):
-        # the key covers every pointer the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
-        # cached table would otherwise keep pointing at the old, freed moment tensors
-        key = tuple((p.data_ptr(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if (st := self.state.get(p)) else (0, 0)))
+        # the key covers every pointer and size the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
+        # cached table would otherwise keep pointing at the old, freed moment tensors, and after p.data = p.data[:k] at elements behind the parameter
+        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if (st := self.state.get(p)) else (0, 0)))
                     for p in ps)
         cached = self._tables.get(gi)
         if cached is not None and cached[0] == key:
@@ -40,13 +40,17 @@ class Adam(torch.optim.Optimizer):
                 st["step"] = 0
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            for s in (p.grad, st["exp_avg"], st["exp_avg_sq"]):
+                if s.shape != p.shape or s.dtype != p.dtype or not s.is_contiguous():
+                    raise RuntimeError("point2cyl_amd.optim.Adam: a gradient or moment of %s %s does not fit its parameter %s"
+                                       % (s.dtype, tuple(s.shape), tuple(p.shape)))
             rows.append([p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()])
             numel.append(p.numel())
             chunks += [[t, c] for c in range((p.numel() + 1023) // 1024)]
         tab = torch.tensor(rows, dtype=torch.int64).to(dev, non_blocking=True)
         nel = torch.tensor(numel, dtype=torch.int64).to(dev, non_blocking=True)
         chk = torch.tensor(chunks, dtype=torch.int32).to(dev, non_blocking=True)
-        key = tuple((p.data_ptr(), p.grad.data_ptr(), self.state[p]["exp_avg"].data_ptr(), self.state[p]["exp_avg_sq"].data_ptr()) for p in ps)
+        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), self.state[p]["exp_avg"].data_ptr(), self.state[p]["exp_avg_sq"].data_ptr()) for p in ps)
         cached = (key, tab, nel, chk, len(chunks), ps)
         self._tables[gi] = cached
         return cached
@@ -124,14 +128,15 @@ class Muon(Adam):
         self._mats = {}
 
     def _matrices(self, gi, ps, group):
-        """Descriptors of the group's matrices, rebuilt when a pointer, the learning rate or the decay changed."""
+        """Descriptors of the group's matrices, rebuilt when a tensor, the learning rate or the decay changed."""
         for p in ps:
             if "momentum_buffer" not in self.state[p]:
                 if torch.cuda.is_current_stream_capturing():       # (the zeros would be part of the graph: every replay would start the momentum again)
                     raise RuntimeError("point2cyl_amd.optim.Muon: take one step before capturing one (a parameter has no momentum yet)")
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
         lr, wd, adjust = float(group["lr"]), float(group["weight_decay"]), group["adjust"]
-        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]), *[(p.data_ptr(), p.grad.data_ptr(), p.grad.stride(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps])
+        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]),
+               *[(t.data_ptr(), t.shape, t.stride(), t.dtype) for p in ps for t in (p, p.grad, self.state[p]["momentum_buffer"])])
         hit = self._mats.get(gi)
         if hit is not None and hit[0] == key:
             return hit

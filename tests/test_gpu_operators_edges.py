@@ -77,3 +77,27 @@ def test_newton_schulz_weak_rows_after_eight_steps(shape, kind):
     floor = min(m, n) * 12.6 * 1.26 * 2.0 ** -38 * sum(NSC[0] ** k for k in range(8))
     assert err(ops.newton_schulz(G, steps=8)) <= 4.0 * err(plain(torch.float32)) + floor
     assert floor <= 4e-5 * want.norm().item()
+
+
+@pytest.mark.parametrize("use_muon", [True, False])
+def test_a_parameter_that_shrank_is_refused(use_muon):
+    """p.data = p.data[:k] keeps every address: the step must not go on with the sizes of the one before."""
+    from point2cyl_amd import optim
+    r = gen(32)
+    for cls, kw in ((optim.Muon, dict(use_muon=use_muon)), (optim.Adam, {})):
+        whole = r(64, 32)
+        p = torch.nn.Parameter(whole)
+        p.grad = r(64, 32)
+        o = cls([dict(params=[p], **kw)], lr=0.01)
+        o.step()
+        grad, keep = p.grad, whole.clone()
+        p.grad = None
+        p.data = whole[:32]
+        p.grad = grad[:32]
+        with pytest.raises(RuntimeError, match="fit|takes"):
+            o.step()
+        assert torch.equal(whole, keep)
+        # with moments of its size the shorter parameter is stepped, what lies behind it stays
+        o.state[p].clear()
+        o.step()
+        assert torch.equal(whole[32:], keep[32:]) and not torch.equal(whole[:32], keep[:32])

@@ -5,7 +5,7 @@ parameters in 123 tensors become ~140 blocks in two launches, 88 us per step on 
 update in a few microseconds.  Here the update of ALL tensors of a parameter group is ONE launch of
 csrc/bn.hip:adam_multi_kernel with 1024-element work items (p2c_adam_multi_f32), driven by a device-resident table of
 (param, grad, exp_avg, exp_avg_sq) pointers.  The table is rebuilt only when a gradient tensor moved (eager steps; under the HIP
-graph the gradient tensors are static).  Same update rule and operation order as torch.optim.Adam (no weight decay, no amsgrad);
+graph the gradient tensors are static), never during a capture; a captured one is kept.  Same update rule and operation order as torch.optim.Adam (no weight decay, no amsgrad);
 `param_groups`, `zero_grad`, `state_dict` keep torch's shapes so schedules that poke `param_groups[i]["lr"]` keep working.
 """
 import ctypes
@@ -19,7 +19,7 @@ from ._lib import call, ptr, stream
 class Adam(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
-        self._tables = {}
+        self._tables, self._captured = {}, []
 
     def _table(self, gi, ps):
         # the key covers every pointer and size the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
@@ -27,8 +27,13 @@ class Adam(torch.optim.Optimizer):
         key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if (st := self.state.get(p)) else (0, 0)))
                     for p in ps)
         cached = self._tables.get(gi)
+        capturing = ps[0].is_cuda and torch.cuda.is_current_stream_capturing()
         if cached is not None and cached[0] == key:
+            if capturing and not any(cached is c for c in self._captured):
+                self._captured.append(cached)          # the graph's replays read this table, also after an eager step with other gradients has replaced it
             return cached
+        if capturing:       # (a copy from host memory that is gone, and zeroed moments, would be part of the graph)
+            raise RuntimeError("point2cyl_amd.optim.%s: take one step with the same gradient tensors before capturing one" % type(self).__name__)
         dev = ps[0].device
         rows, numel, chunks = [], [], []
         for t, p in enumerate(ps):
@@ -100,13 +105,14 @@ class Muon(Adam):
     group with use_muon=False, take Adam's rule with the group's `betas` and `adam_eps` in one launch, without decay.
 
     fp32, contiguous; `param_groups`, `state_dict` keep torch's shapes (state: "momentum_buffer" for matrices, Adam's three for the others).  A step can
-    be captured into a graph after one eager step has made the state; its replays keep the learning rates (and Adam's step count) of the capture."""
+    be captured into a graph after one eager step has made the state - where vectors take part, with the same gradient tensors; its replays keep the learning
+    rates (and Adam's step count) of the capture and need the optimizer's state, so the optimizer has to stay."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, ns_coeffs=ops.NS_COEFFS, eps=1e-7, adjust="rms",
                  betas=(0.9, 0.999), adam_eps=1e-8, use_muon=True):
         torch.optim.Optimizer.__init__(self, params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
                                                           ns_coeffs=ns_coeffs, eps=eps, adjust=adjust, betas=betas, adam_eps=adam_eps, use_muon=use_muon))
-        self._tables, self._mats = {}, {}
+        self._tables, self._captured, self._mats = {}, [], {}
 
     @staticmethod
     def _check_group(g):

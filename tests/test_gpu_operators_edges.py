@@ -101,3 +101,51 @@ def test_a_parameter_that_shrank_is_refused(use_muon):
         o.state[p].clear()
         o.step()
         assert torch.equal(whole[32:], keep[32:]) and not torch.equal(whole[:32], keep[:32])
+
+
+@pytest.mark.parametrize("name", ["Muon", "Adam"])
+def test_captured_step_survives_steps_with_other_gradients(name):
+    """Vectors go by a table in device memory: the one a graph was captured with stays when an eager step makes another."""
+    from point2cyl_amd import optim
+    r = gen(33)
+    make = lambda ps: getattr(optim, name)(ps, lr=0.01)  # noqa: E731
+    base = [r(300), r(64, 48), r(5)]
+    ps, qs = ([torch.nn.Parameter(t.clone()) for t in base] for _ in range(2))
+    g0, g1 = ([r(*t.shape) for t in base] for _ in range(2))
+    o, o2 = make(ps), make(qs)
+    give = lambda ts, gs: [setattr(t, "grad", g) for t, g in zip(ts, gs)]  # noqa: E731
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        give(ps, g0), o.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            o.step()
+        moved = [g.clone() for g in g0]
+        give(ps, moved)
+        with pytest.raises(RuntimeError, match="same gradient tensors"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=st):
+            make(ps).step() if name == "Adam" else o.step()
+        give(ps, g0)
+    torch.cuda.synchronize()
+    counts = {p: o.state[p]["step"] for p in ps if "step" in o.state[p]}
+    step = max(counts.values())                                  # of the capture: what every replay takes for the bias correction
+    give(qs, g0), o2.step()
+
+    def replayed():
+        for q in qs:
+            if "step" in o2.state[q]:
+                o2.state[q]["step"] = step - 1
+        give(qs, g0), o2.step()
+    for k in range(4):
+        graph.replay(), replayed()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
+        for t, oo in ((ps, o), (qs, o2)):                         # an eager step with other gradient tensors
+            for p in t:
+                if "step" in oo.state[p]:
+                    oo.state[p]["step"] = 10 + k
+            give(t, g1), oo.step()
+        junk = [torch.full((n,), -1, dtype=torch.int64, device="cuda") for n in (8, 16, 64, 512, 4096) for _ in range(20)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
+        del junk

@@ -40,6 +40,8 @@ class Adam(torch.optim.Optimizer):
             _lib.require_device(p, p.grad)
             if p.dtype != torch.float32 or not p.is_contiguous() or not p.grad.is_contiguous():
                 raise RuntimeError("point2cyl_amd.optim.Adam takes contiguous fp32 parameters and gradients")
+            if p.device != dev or p.grad.device != dev:
+                raise RuntimeError("point2cyl_amd.optim.Adam: the parameters of a group are on one device (got %s and %s)" % (dev, p.device))
             st = self.state[p]
             if not st:
                 st["step"] = 0
@@ -81,16 +83,18 @@ class Adam(torch.optim.Optimizer):
         return loss
 
     def _adam(self, gi, ps, lr, betas, eps):
-        _, tab, nel, chk, n_chunks, ps = self._table(gi, ps)
-        for p in ps:
-            self.state[p]["step"] += 1
-        steps = {int(self.state[p]["step"]) for p in ps}
-        if len(steps) != 1:     # one bias correction per launch: every tensor of the group must have taken the same number of updates
-            raise RuntimeError("point2cyl_amd.optim.Adam: parameters of one group have different step counts %s (a parameter that first "
-                               "received a gradient later than the others); put it in its own param group" % sorted(steps))
-        b1, b2 = betas
-        call("p2c_adam_multi_f32", ptr(tab), ptr(nel), ptr(chk), n_chunks, float(lr), float(b1), float(b2), float(eps),
-             int(self.state[ps[0]]["step"]), stream())
+        _lib.require_device(ps[0])
+        with _lib.on(ps[0].device):
+            _, tab, nel, chk, n_chunks, ps = self._table(gi, ps)
+            for p in ps:
+                self.state[p]["step"] += 1
+            steps = {int(self.state[p]["step"]) for p in ps}
+            if len(steps) != 1:     # one bias correction per launch: every tensor of the group must have taken the same number of updates
+                raise RuntimeError("point2cyl_amd.optim.Adam: parameters of one group have different step counts %s (a parameter that first "
+                                   "received a gradient later than the others); put it in its own param group" % sorted(steps))
+            b1, b2 = betas
+            call("p2c_adam_multi_f32", ptr(tab), ptr(nel), ptr(chk), n_chunks, float(lr), float(b1), float(b2), float(eps),
+                 int(self.state[ps[0]]["step"]), stream())
 
 
 class Muon(Adam):

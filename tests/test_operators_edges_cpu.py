@@ -42,3 +42,34 @@ def test_newton_schulz_refuses_steps_that_amplify_too_much():
         assert entry(len(co), co) == -1, co
     with pytest.raises(ValueError, match="2\\^15"):
         optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], ns_steps=16)
+
+
+@pytest.mark.parametrize("name", ["Adam", "Muon"])
+def test_adams_rule_runs_on_the_parameters_device(name, monkeypatch):
+    """The launch (and its stream) belong to the device of the group's parameters, not to the current one."""
+    seen, inside = [], []
+
+    class On:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            inside.append(self.device)
+
+        def __exit__(self, *a):
+            inside.pop()
+    monkeypatch.setattr(_lib, "require_device", lambda *t: None)
+    monkeypatch.setattr(_lib, "on", On)
+    monkeypatch.setattr(optim, "stream", lambda: 0)
+    monkeypatch.setattr(optim, "call", lambda f, *a, **k: seen.append((f, list(inside))))
+    p = torch.nn.Parameter(torch.zeros(5))
+    p.grad = torch.ones(5)
+    o = getattr(optim, name)([p])
+    o.step()
+    assert seen == [("p2c_adam_multi_f32", [p.device])] and not inside
+    q = torch.nn.Parameter(torch.zeros(3, device="meta"))
+    q.grad = torch.ones(3, device="meta")
+    o.add_param_group({"params": [q]})
+    o.param_groups[0]["params"].append(q)
+    with pytest.raises(RuntimeError, match="one device"):
+        o.step()

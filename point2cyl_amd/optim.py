@@ -24,7 +24,7 @@ class Adam(torch.optim.Optimizer):
     def _table(self, gi, ps):
         # the key covers every pointer and size the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
         # cached table would otherwise keep pointing at the old, freed moment tensors, and after p.data = p.data[:k] at elements behind the parameter
-        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if (st := self.state.get(p)) else (0, 0)))
+        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if "exp_avg" in (st := self.state.get(p, ())) else (0, 0)))
                     for p in ps)
         cached = self._tables.get(gi)
         capturing = ps[0].is_cuda and torch.cuda.is_current_stream_capturing()
@@ -43,7 +43,7 @@ class Adam(torch.optim.Optimizer):
             if p.device != dev or p.grad.device != dev:
                 raise RuntimeError("point2cyl_amd.optim.Adam: the parameters of a group are on one device (got %s and %s)" % (dev, p.device))
             st = self.state[p]
-            if not st:
+            if "exp_avg" not in st:        # (a matrix whose group left Muon's rule has its momentum here)
                 st["step"] = 0
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)

@@ -73,3 +73,20 @@ def test_adams_rule_runs_on_the_parameters_device(name, monkeypatch):
     o.param_groups[0]["params"].append(q)
     with pytest.raises(RuntimeError, match="one device"):
         o.step()
+
+
+def test_a_group_can_leave_muons_rule(monkeypatch):
+    """A matrix that has a momentum and no moments yet takes Adam's rule from then on."""
+    seen = []
+    monkeypatch.setattr(_lib, "require_device", lambda *t: None)
+    monkeypatch.setattr(_lib, "on", lambda d: _lib._HERE_ALREADY)
+    monkeypatch.setattr(optim, "stream", lambda: 0)
+    monkeypatch.setattr(optim, "call", lambda f, *a, **k: seen.append(f))
+    p = torch.nn.Parameter(torch.zeros(5, 4))
+    p.grad = torch.ones(5, 4)
+    o = optim.Muon([p])
+    o.state[p]["momentum_buffer"] = torch.zeros(5, 4)
+    o.param_groups[0]["use_muon"] = False
+    o.step()
+    o.step()
+    assert seen == ["p2c_adam_multi_f32"] * 2 and o.state[p]["step"] == 2 and set(o.state[p]) == {"momentum_buffer", "step", "exp_avg", "exp_avg_sq"}

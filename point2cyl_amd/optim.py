@@ -62,9 +62,10 @@ class Adam(torch.optim.Optimizer):
         self._tables[gi] = cached
         return cached
 
-    def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+    def __setstate__(self, state):         # copies, pickles and load_state_dict come through here; tables of captured steps stay with their optimizer
+        super().__setstate__(state)
         self._tables = {}
+        self.__dict__.setdefault("_captured", [])
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -128,8 +129,8 @@ class Muon(Adam):
             raise ValueError("Muon: eps = %r has to be positive" % (g["eps"],))
         ops.ns_coefficients(g["ns_steps"], g["ns_coeffs"])
 
-    def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+    def __setstate__(self, state):
+        super().__setstate__(state)
         self._mats = {}
 
     def add_param_group(self, param_group):

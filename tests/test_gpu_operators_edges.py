@@ -149,3 +149,25 @@ def test_captured_step_survives_steps_with_other_gradients(name):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
         del junk
+
+
+@pytest.mark.parametrize("name", ["Muon", "Adam"])
+def test_a_copied_optimizer_goes_on_alone(name):
+    from point2cyl_amd import optim
+    r = gen(34)
+    ps = [torch.nn.Parameter(r(60, 40)), torch.nn.Parameter(r(7))]
+    o = getattr(optim, name)(ps, lr=0.01)
+    gs = [[r(*p.shape) for p in ps] for _ in range(4)]
+
+    def steps(opt, some):
+        for g in some:
+            for p, d in zip(opt.param_groups[0]["params"], g):
+                p.grad = d.clone()
+            opt.step()
+    steps(o, gs[:2])
+    c = copy.deepcopy(o)
+    keep = [p.detach().clone() for p in ps]
+    steps(c, gs[2:])
+    assert all(torch.equal(p, k) for p, k in zip(ps, keep))
+    steps(o, gs[2:])
+    assert all(torch.equal(p, q) and not torch.equal(p, k) for p, q, k in zip(ps, c.param_groups[0]["params"], keep))

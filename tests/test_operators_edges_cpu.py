@@ -1,5 +1,7 @@
 """CPU: the ends of what the dense-layer operators accept - launch sizes, row counts, settings - and what they refuse there."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -90,3 +92,19 @@ def test_a_group_can_leave_muons_rule(monkeypatch):
     o.step()
     o.step()
     assert seen == ["p2c_adam_multi_f32"] * 2 and o.state[p]["step"] == 2 and set(o.state[p]) == {"momentum_buffer", "step", "exp_avg", "exp_avg_sq"}
+
+
+@pytest.mark.parametrize("name", ["Adam", "Muon"])
+def test_optimizers_can_be_copied_and_pickled(name):
+    p = torch.nn.Parameter(torch.zeros(5, 4))
+    o = getattr(optim, name)([p], lr=0.5)
+    o._captured.append("a captured step's table")
+    for c in (copy.deepcopy(o), pickle.loads(pickle.dumps(o))):
+        assert type(c) is type(o) and c.param_groups[0]["lr"] == 0.5 and c._tables == {} and c._captured == []
+        assert name == "Adam" or c._mats == {}
+        c.param_groups[0]["params"][0].grad = torch.ones(5, 4)
+        with pytest.raises(RuntimeError, match="no CPU path"):       # (as far as a step gets here)
+            c.step()
+    o._tables[0] = "old"
+    o.load_state_dict(o.state_dict())
+    assert o._tables == {} and o._captured

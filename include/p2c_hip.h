@@ -602,8 +602,8 @@ int p2c_muon_step_f32(const p2c_ns_matrix *mats_host, int n, float momentum, int
  *     q = 0.  A row below 2^-119 throughout: s = 0, q = 0.  ldx: row stride of x in elements (the columns are contiguous).  More than
  *     p2c_quantize_rows_at_once(K) rows take several launches.
  *   p2c_int8_linear: out[r][n] = act((sum_k xq wq) sx[r] sw[n] + bias[n] + add[r][n]); act 0 none, 1 ReLU, 2 softplus(beta, thr); bias, add may be NULL.
- *   p2c_int8_linear_requant (N <= 512; softplus: thr >= 17): the same result as quantised rows out [M][ldo = p2c_int8_padded(N)], so [M]; the fp32
- *     values never reach memory.
+ *   p2c_int8_linear_requant (N <= 512; softplus: thr >= 17, beta >= 0.7): the same result as quantised rows out [M][ldo = p2c_int8_padded(N)], so [M];
+ *     the fp32 values never reach memory.  With softplus a row that reaches 2^127 / beta counts as infinite.
  *   p2c_int8_linear_few (M <= 32, K <= 2048): x as floats of xdtype, quantised in the same launch.
  *   p2c_int8_linear_float, _requant_float: x as floats, any M; ws: M * Kp + 4 M bytes, 16-byte aligned (the quantised rows; NULL where
  *     p2c_int8_few_supported for _float). */

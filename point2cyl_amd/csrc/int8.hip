@@ -765,6 +765,7 @@ extern "C" int p2c_int8_padded(int K) { return K < 1 ? 0 : (K + 63) / 64 * 64; }
 extern "C" int p2c_int8_padded_out(int N) { return N < 1 ? 0 : (N + 255) / 256 * 256; }
 extern "C" int p2c_int8_few_supported(int M, int K) { return M >= 1 && M <= 32 && K >= 1 && K <= 2048; }
 // (the epilogue's softplus has no linear region of its own: above beta x = 17 it is the identity in 32 bits anyway, so the threshold has to lie there)
+// The epilogue works in units of log2(e) / beta, and its rows have to keep their normal range there: beta >= 0.7 (unit >= 1; checked at the entry).
 extern "C" int p2c_int8_requant_supported(int N, int act, float thr) { return N >= 1 && N <= 512 && (act != 2 || thr >= 17.0f); }
 
 extern "C" int p2c_quantize_rows_at_once(int K) { return K < 1 ? 0 : quantize_rows_at_once(p2c_int8_padded(K)); }
@@ -832,7 +833,7 @@ extern "C" int p2c_int8_linear_requant(const int8_t *xq, long long ldx, const fl
                                        const float *add, long long ldadd, int act, float beta, float thr, int8_t *out, int ldo, float *so, int M, int N, int K,
                                        int Kp, void *stream)
 {
-    if (i8_shape_bad(M, K, Kp) || !p2c_int8_requant_supported(N, act, thr) || ldx < Kp || ldx > I8_MAX_LD || ldo != (N + 63) / 64 * 64) return P2C_EINVAL;
+    if (i8_shape_bad(M, K, Kp) || !p2c_int8_requant_supported(N, act, thr) || (act == 2 && !(beta >= 0.7f)) || ldx < Kp || ldx > I8_MAX_LD || ldo != (N + 63) / 64 * 64) return P2C_EINVAL;
     I8Epi e;
     const int rc = i8_epilogue(e, sx, sw, bias, add, ldadd, act, beta, thr, out, ldo, 0, N);
     if (rc != P2C_OK) return rc;

@@ -1793,7 +1793,7 @@ def linear_int8(x, w, act="none", beta=100.0, threshold=20.0, add=None, out_dtyp
             few = L.p2c_int8_few_supported(M, K) and not requantize
             ws = None if few else torch.empty(M * (w.Kp + 4), dtype=torch.int8, device=dev)
             xin = (ptr(x), _DTYPES[x.dtype], x.stride(0) if M > 1 else K)
-        if requantize and L.p2c_int8_requant_supported(w.N, _INT8_ACTS[act], float(threshold)):
+        if requantize and L.p2c_int8_requant_supported(w.N, _INT8_ACTS[act], float(threshold)) and (act != "softplus" or beta >= 0.75):
             ldo = (w.N + 63) // 64 * 64
             q = torch.empty(M, ldo, dtype=torch.int8, device=dev)
             so = torch.empty(M, dtype=torch.float32, device=dev)

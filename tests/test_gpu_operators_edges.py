@@ -171,3 +171,25 @@ def test_a_copied_optimizer_goes_on_alone(name):
     assert all(torch.equal(p, k) for p, k in zip(ps, keep))
     steps(o, gs[2:])
     assert all(torch.equal(p, q) and not torch.equal(p, k) for p, q, k in zip(ps, c.param_groups[0]["params"], keep))
+
+
+@pytest.mark.parametrize("beta", [0.01, 0.5, 0.75, 1.0, 100.0])
+def test_requantised_softplus_far_below_zero(beta):
+    """Arguments z with beta z from -80 to -86: values of e^(beta z) / beta, down to 2^-124 / beta, next to the end of the range.  The rows given back are within half a quantum of the
+    floats (plus their relative error: 2^-22 beta |z| on either side), rows below 2^-119 are zero."""
+    from point2cyl_amd import ops
+    r = gen(35)
+    M, K, N = 70, 64, 40
+    w = ops.Int8Weight(1e-3 * r(N, K) / beta, torch.full((N,), -80.0 / beta, device="cuda"))
+    x = r(M, K)
+    add = -torch.linspace(0, 6, M, device="cuda")[:, None].expand(M, N).contiguous() / beta
+    y = ops.linear_int8(x, w, act="softplus", beta=beta, add=add)
+    h = ops.linear_int8(x, w, act="softplus", beta=beta, add=add, requantize=True)
+    top = y.abs().amax(1)
+    live = top > 2.0 ** -118
+    assert (h.scale[live] > 0).all() and (h.scale[top < 2.0 ** -120] == 0).all()
+    assert bool(live.any()) == (beta < 100.0)                    # (e^-80 / 100 = 1.8e-37 is below 2^-119 = 1.5e-36 already)
+    s = h.scale.double()[:, None]
+    off = (h.q.double() * s - y.double()).abs()
+    assert (off <= 0.5001 * s + 2.0 ** -21 * 87 * y.double())[live].all()
+    assert (h.q.abs().amax(1) >= 126)[live].all() and not h.q[h.scale == 0].any()

@@ -108,3 +108,11 @@ def test_optimizers_can_be_copied_and_pickled(name):
     o._tables[0] = "old"
     o.load_state_dict(o.state_dict())
     assert o._tables == {} and o._captured
+
+
+def test_requantising_softplus_refuses_a_small_beta():
+    """Its epilogue holds the rows times 1.44 beta: below 0.7 a row in the normal range would leave it there (ops.linear_int8 takes the unfused form)."""
+    L = _lib.lib()
+    entry = lambda act, beta: L.p2c_int8_linear_requant(ONE, 64, ONE, ONE, ONE, None, None, 0, act, beta, 20.0, ONE, 64, ONE, 0, 8, 8, 64, None)  # noqa: E731
+    assert entry(2, 100.0) == 0 and entry(2, 0.75) == 0 and entry(1, 0.01) == 0
+    assert entry(2, 0.69) == -1 and entry(2, 0.01) == -1 and entry(2, float("nan")) == -1

@@ -576,7 +576,7 @@ int p2c_eval_metrics_f32(const float *heads, int ld, int xoff, int woff, const f
  *     U = nesterov ? (1 - momentum) G + momentum mom : mom;  dst = decay dst - scale newton_schulz(U).
  * The coefficients have to keep every |X| below 3.8 and the polynomial below 15 from a start of 1, and the steps from any one to the last may amplify
  * weak directions by 2^15 at most (the product of their largest |a + b x^2 + c x^4|; the accuracy would not hold beyond): P2C_EINVAL otherwise.
- * steps 1 ... 16, eps > 0.
+ * steps 1 ... 16, eps > 0 and finite.
  * ws: 16-byte aligned, p2c_newton_schulz_ws_bytes of the same descriptors, no initialisation; not shared by calls that may run at the same time.
  * ------------------------------------------------------------------------------------------- */
 typedef struct p2c_ns_matrix {

@@ -178,6 +178,10 @@ __device__ __forceinline__ void ns_load_tile(const NsTab &a, const NsMat &d, con
     for (int q = 0; q < 16; ++q) v[q] = ok(q) ? v[q] : 0.f;
 }
 
+// what brings a matrix whose squares sum to s to unit norm.  A zero matrix stays zero whatever eps is (1 / eps may leave 64 bits); any other 32-bit matrix has a norm
+// of 2^-149 at least.
+__device__ __forceinline__ double ns_unit(double s, double eps) { return s == 0.0 ? 1.0 : 1.0 / (sqrt(s) + eps); }
+
 // partial sums of a matrix: one per 64 x 64 tile of it, at most NS_PARTS
 __host__ __device__ __forceinline__ int ns_parts(int m, int n)
 {
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(256) ns_begin_kernel(const NsTab a)
     s = p2c_wave_sum_f64(s);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
-    const double inv = (double)NS_SCALE / (sqrt(red[0] + red[1] + red[2] + red[3]) + a.eps);
+    const double inv = (double)NS_SCALE * ns_unit(red[0] + red[1] + red[2] + red[3], a.eps);
 #pragma unroll
     for (int q = 0; q < 16; ++q) x[(tid >> 6) + 4 * q][tid & 63] = (float)((double)v[q] * inv);
     __syncthreads();
@@ -657,7 +661,7 @@ __global__ void __launch_bounds__(512) ns_mid_kernel(const NsTab a, const NsCoef
     s = 0.0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) s += red[k];
-    const double inv = (double)NS_SCALE / (sqrt(s) + a.eps);
+    const double inv = (double)NS_SCALE * ns_unit(s, a.eps);
     const float finv = (float)inv;
     if (finv > 1e-30f && finv < 1e30f) {                        // the factor of ordinary magnitudes is a 32-bit number
 #pragma unroll
@@ -967,7 +971,7 @@ __device__ __forceinline__ void ns_small(const NsTab &a, const NsCoef &co, int m
     double tr = 0.0;
 #pragma unroll
     for (int k = 0; k < M; ++k) tr += l.A[k][k];
-    const double inv = 1.0 / (sqrt(tr) + a.eps);
+    const double inv = ns_unit(tr, a.eps);
     __syncthreads();
     if (on) {
         l.A[ei][ej] *= inv * inv;
@@ -1225,7 +1229,7 @@ int ns_run(const p2c_ns_matrix *mats, int n, int dtype, float mu, int muon, int 
 {
     const int rc = ns_check(mats, n);
     if (rc != P2C_OK) return rc;
-    if (steps < 1 || steps > 16 || !coeffs || !(eps > 0.0) || dtype < 0 || dtype > 2) return P2C_EINVAL;
+    if (steps < 1 || steps > 16 || !coeffs || !(eps > 0.0) || !isfinite(eps) || dtype < 0 || dtype > 2) return P2C_EINVAL;
     NsCoef co;
     co.steps = steps;
     // every matrix of the iteration has to stay inside the range of the scaled fp16 pairs: follow the bound of the spectrum

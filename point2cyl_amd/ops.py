@@ -1606,8 +1606,8 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     items = list(G) if many else [G]
     if not items:
         return []
-    if not eps > 0.0:
-        raise ValueError("newton_schulz: eps = %r has to be positive" % (eps,))
+    if not 0.0 < eps < float("inf"):
+        raise ValueError("newton_schulz: eps = %r has to be positive and finite" % (eps,))
     co = ns_coefficients(steps, coeffs)
     dev = items[0].device
     groups, outs = {}, []

@@ -125,8 +125,8 @@ class Muon(Adam):
             raise ValueError("Muon: momentum = %r is outside [0, 1)" % (g["momentum"],))
         if g["adjust"] not in ("rms", "spectral"):
             raise ValueError("Muon: adjust %r is neither rms nor spectral" % (g["adjust"],))
-        if not g["eps"] > 0.0:
-            raise ValueError("Muon: eps = %r has to be positive" % (g["eps"],))
+        if not 0.0 < g["eps"] < float("inf"):
+            raise ValueError("Muon: eps = %r has to be positive and finite" % (g["eps"],))
         ops.ns_coefficients(g["ns_steps"], g["ns_coeffs"])
 
     def __setstate__(self, state):

@@ -193,3 +193,28 @@ def test_requantised_softplus_far_below_zero(beta):
     off = (h.q.double() * s - y.double()).abs()
     assert (off <= 0.5001 * s + 2.0 ** -21 * 87 * y.double())[live].all()
     assert (h.q.abs().amax(1) >= 126)[live].all() and not h.q[h.scale == 0].any()
+
+
+@pytest.mark.parametrize("shape", [(5, 70), (16, 16), (80, 90), (300, 200)])
+@pytest.mark.parametrize("eps", [1e-30, 1e-80, 1e-160, 1e-310])
+def test_newton_schulz_zero_matrix_and_a_tiny_eps(shape, eps):
+    """Every kernel: zeros stay zeros and do not touch their neighbours; the smallest matrices that are not zero go by the formula (where eps outweighs their norm they stay small).
+    Bound: 2^-20 of every step's result and the operands' floor, carried on by at most 3.4445 a step (as in the other tests of these kernels)."""
+    from point2cyl_amd import ops
+    G = torch.zeros(3, *shape, device="cuda")
+    G[1] = gen(36)(*shape)
+    G[2] = G[1].sign() * 2.0 ** -140                        # (subnormal)
+    o = ops.newton_schulz(G, eps=eps)
+    assert not o[0].any()
+    m = min(shape)
+    for k in (1, 2):
+        X = G[k].double()
+        X = X / (X.norm() + eps)
+        X = X.t().contiguous() if shape[0] > shape[1] else X
+        bound = 2.0 ** -20 * X.norm().item()
+        for _ in range(5):
+            A = X @ X.t().contiguous()
+            X = NSC[0] * X + (NSC[1] * A + NSC[2] * (A @ A)) @ X
+            bound = NSC[0] * bound + 2.0 ** -20 * X.norm().item() + m * 12.6 * 1.26 * 2.0 ** -38
+        X = X.t() if shape[0] > shape[1] else X
+        assert (o[k].double() - X).norm().item() <= bound, k

@@ -116,3 +116,16 @@ def test_requantising_softplus_refuses_a_small_beta():
     entry = lambda act, beta: L.p2c_int8_linear_requant(ONE, 64, ONE, ONE, ONE, None, None, 0, act, beta, 20.0, ONE, 64, ONE, 0, 8, 8, 64, None)  # noqa: E731
     assert entry(2, 100.0) == 0 and entry(2, 0.75) == 0 and entry(1, 0.01) == 0
     assert entry(2, 0.69) == -1 and entry(2, 0.01) == -1 and entry(2, float("nan")) == -1
+
+
+def test_newton_schulz_refuses_an_infinite_eps():
+    L = _lib.lib()
+    co = ops.ns_coefficients(5, ops.NS_COEFFS)
+    m = (_lib.NsMatrix * 1)()
+    m[0].rows, m[0].cols, m[0].batch = 0, 4, 1
+    for eps, rc in ((1e-7, 0), (1e-300, 0), (float("inf"), -1), (0.0, -1)):
+        assert L.p2c_newton_schulz(m, 1, 0, 5, co, eps, ONE, 1 << 20, None) == rc
+    with pytest.raises(ValueError, match="finite"):
+        optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], eps=float("inf"))
+    with pytest.raises(ValueError, match="finite"):
+        ops.newton_schulz([torch.zeros(4, 4)], eps=float("inf"))

@@ -1082,11 +1082,12 @@ inline size_t ns_one_ws(const p2c_ns_matrix &m, int tile)
     return NS_PARTS * 8 + 3 * ns_xbytes(mP, nP) + 2 * ns_xbytes(mP, mP);
 }
 
+// sides up to 2^23 (the byte offset of a tile's rows in a block of 32 k has 32 bits), 65536 matrices per descriptor (a launch's workgroups)
 int ns_check(const p2c_ns_matrix *mats, int n)
 {
     if (!mats || n <= 0) return P2C_EINVAL;
     for (int i = 0; i < n; ++i)
-        if (mats[i].rows < 0 || mats[i].cols < 0 || mats[i].batch < 0 || mats[i].rows > (1 << 20) || mats[i].cols > (1 << 20) ||
+        if (mats[i].rows < 0 || mats[i].cols < 0 || mats[i].batch < 0 || mats[i].rows > (1 << 23) || mats[i].cols > (1 << 23) ||
             (long long)mats[i].rows * mats[i].cols > (1ll << 31) || mats[i].batch > (1 << 16)) return P2C_EINVAL;
     return P2C_OK;
 }

@@ -1583,6 +1583,14 @@ def _ns_coefficients(steps, coeffs):
     return (ctypes.c_float * (3 * steps))(*[v for r in rows for v in r])
 
 
+_NS_SIDE, _NS_ELEMENTS, _NS_BATCH = 1 << 23, 1 << 31, 1 << 16      # a matrix' sides and elements, the matrices of one descriptor (csrc/muon.hip)
+
+
+def ns_check_size(r, c, what):
+    if max(r, c) > _NS_SIDE or r * c > _NS_ELEMENTS:
+        raise ValueError("%s: sides up to 2^23 and 2^31 elements, got a matrix of %d x %d" % (what, r, c))
+
+
 def _ns_record(src, dst):
     """One matrix (or batch of equal ones) as a p2c_ns_matrix; the layout along which the columns are contiguous is the one the kernels read best."""
     r, c = src.shape[-2], src.shape[-1]
@@ -1596,10 +1604,10 @@ def _ns_record(src, dst):
 def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """The orthogonalised form of a matrix (r, c), of every matrix of a batch (..., r, c), or of every matrix of a list (any shapes, one device):
     X_0 = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T of the smaller side - all singular values are driven
-    towards 1, the singular vectors stay.  fp32, bf16 or fp16, any strides; 32-bit accuracy inside whatever the type, one rounding at the end.
-    Steps that together amplify the weakest directions by more than 2^15 are refused (up to eight of the default coefficients are taken): beyond that
-    rows 1e-9 of the others, which 32-bit numbers keep, would be lost.  The path goes by the whole call,
-    so a matrix may differ in its last bits alone and in a list.
+    towards 1, the singular vectors stay.  fp32, bf16 or fp16, any strides, sides up to 2^23 and 2^31 elements; 32-bit accuracy inside whatever the
+    type, one rounding at the end.  Steps that together amplify the weakest directions by more than 2^15 are refused (up to eight of the default
+    coefficients are taken): beyond that rows 1e-9 of the others, which 32-bit numbers keep, would be lost.  The path goes by the whole call, so a
+    matrix may differ in its last bits alone and in a list.
     A zero matrix gives zeros; a matrix that holds an infinity or a NaN gives NaN (others of the call are not touched).  The result is
     contiguous and has no gradient.  Reference use: an update rule beside torch.optim.Adam (train_Point2Cyl_without_sketch.py:204)."""
     many = not isinstance(G, torch.Tensor)
@@ -1625,8 +1633,13 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         outs.append(o)
         if g.numel():
             src, dst = (g, o) if g.dim() == 2 else (g.reshape(-1, *g.shape[-2:]), o.view(-1, *g.shape[-2:]))
+            ns_check_size(*src.shape[-2:], "newton_schulz")
             # (bound to `src` until the launch: reshape may have made a copy)
-            groups.setdefault(_DTYPES[g.dtype], []).append((src, _ns_record(src, dst)))
+            mine = groups.setdefault(_DTYPES[g.dtype], [])
+            if src.dim() == 2:
+                mine.append((src, _ns_record(src, dst)))
+            else:
+                mine += [(src, _ns_record(src[b:b + _NS_BATCH], dst[b:b + _NS_BATCH])) for b in range(0, src.shape[0], _NS_BATCH)]
     with _lib.on(dev):
         for dt, recs in groups.items():
             buf = b"".join(r for _, r in recs)
@@ -1700,8 +1713,8 @@ def _int8_rows_in(x, what):
 
 
 def quantize_rows(x):
-    """Rows (M, K) of fp32, bf16 or fp16, M up to 2^30 - 64, K up to 131072 -> Int8Rows with a scale each: scale = max |row| * (1 / 127) in fp32, q = x / scale rounded to the nearest whole
-    number, ties to even (of the exact quotient).  A row that holds an infinity or a NaN has scale NaN and q = 0 (its products are NaN, the
+    """Rows (M, K) of fp32, bf16 or fp16 (M up to 2^30 - 64, K up to 131072) -> Int8Rows with a scale each: scale = max |row| * (1 / 127) in fp32,
+    q = x / scale rounded to the nearest whole number, ties to even (of the exact quotient).  A row that holds an infinity or a NaN has scale NaN and q = 0 (its products are NaN, the
     other rows are not touched); a row whose magnitudes are all below 2^-119 is a row of zeros."""
     x = _int8_rows_in(x, "quantize_rows")
     M, K = x.shape

@@ -164,6 +164,7 @@ class Muon(Adam):
             c = p.numel() // r if r else 0
             if not p.numel():
                 continue
+            ops.ns_check_size(r, c, "point2cyl_amd.optim.Muon")
             s = 0.2 * max(r, c) ** 0.5 if adjust == "rms" else max(1.0, r / c) ** 0.5
             recs.append(ops._NS_RECORD.pack(p.grad.data_ptr(), m.data_ptr(), p.data_ptr(), c, 1, 0, c, 1, 0, r, c, 1, lr * s, 1.0 - lr * wd))
         buf = ctypes.create_string_buffer(b"".join(recs), max(1, len(recs) * ops._NS_RECORD.size))

@@ -218,3 +218,44 @@ def test_newton_schulz_zero_matrix_and_a_tiny_eps(shape, eps):
             bound = NSC[0] * bound + 2.0 ** -20 * X.norm().item() + m * 12.6 * 1.26 * 2.0 ** -38
         X = X.t() if shape[0] > shape[1] else X
         assert (o[k].double() - X).norm().item() <= bound, k
+
+
+def ns64(G):
+    """-> (result in 64 bits, bound on the Frobenius error: 2^-20 of every step's result, carried on, and half a unit of the type)"""
+    X = G.double()
+    X = X / (X.norm() + 1e-7)
+    X = X.t() if G.shape[0] > G.shape[1] else X
+    bound = 2.0 ** -20 * X.norm().item()
+    for _ in range(5):
+        A = X @ X.t().contiguous()
+        X = NSC[0] * X + (NSC[1] * A + NSC[2] * (A @ A)) @ X.contiguous()
+        bound = NSC[0] * bound + 2.0 ** -20 * X.norm().item()
+    return X.t() if G.shape[0] > G.shape[1] else X, bound + {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[G.dtype] * X.norm().item()
+
+
+@pytest.mark.parametrize("shape,dtype", [((70000, 3, 3), torch.float32), ((65537, 20, 24), torch.bfloat16), ((2, 131075, 6), torch.float32)])
+def test_newton_schulz_batches_larger_than_a_descriptor(shape, dtype):
+    from point2cyl_amd import ops
+    G = gen(37)(*shape).to(dtype)
+    o = ops.newton_schulz(G)
+    for k in {0, 1, 65535, 65536, shape[0] - 1}:
+        if k < shape[0]:
+            want, bound = ns64(G[k])
+            assert (o[k].double() - want).norm().item() <= bound, k
+    v = G.transpose(-1, -2)
+    lo = max(0, shape[0] - 5)
+    assert torch.equal(ops.newton_schulz(v)[lo:], ops.newton_schulz(v[lo:]))
+
+
+@pytest.mark.parametrize("shape,dtype", [((3, 2000000), torch.float32), ((1200000, 64), torch.bfloat16), ((20, (1 << 20) + 33), torch.float32)])
+def test_newton_schulz_and_muon_on_very_long_matrices(shape, dtype):
+    from point2cyl_amd import ops, optim
+    G = gen(38)(*shape).to(dtype)
+    want, bound = ns64(G)
+    assert (ops.newton_schulz(G).double() - want).norm().item() <= bound
+    if dtype == torch.float32:
+        p = torch.nn.Parameter(torch.zeros_like(G))
+        p.grad = G
+        optim.Muon([p], lr=1.0, momentum=0.0, adjust="spectral").step()
+        scale = max(1.0, shape[0] / shape[1]) ** 0.5
+        assert (p.detach().double() + scale * want).norm().item() <= scale * bound

@@ -129,3 +129,19 @@ def test_newton_schulz_refuses_an_infinite_eps():
         optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], eps=float("inf"))
     with pytest.raises(ValueError, match="finite"):
         ops.newton_schulz([torch.zeros(4, 4)], eps=float("inf"))
+
+
+def test_newton_schulz_size_limits():
+    L = _lib.lib()
+
+    def need(r, c, batch=1):
+        m = (_lib.NsMatrix * 1)()
+        m[0].rows, m[0].cols, m[0].batch, m[0].src, m[0].dst = r, c, batch, 16, 16
+        return L.p2c_newton_schulz_ws_bytes(m, 1)
+    # padded sides, three images of X, two of the small side's square
+    assert need(64, 1 << 23) >= 3 * 4 * 64 << 23 and need(1 << 23, 256) >= 3 * 4 * 256 << 23
+    assert need(64, (1 << 23) + 1) == 0 and need(300, 1 << 23) == 0 and need(64, 200, (1 << 16) + 1) == 0 and need(64, 2000, 1 << 16) > 0
+    for r, c in ((1, (1 << 23) + 1), (1 << 23, 257), ((1 << 31) + 7, 1)):
+        with pytest.raises(ValueError, match="2\\^23"):
+            ops.ns_check_size(r, c, "x")
+    ops.ns_check_size(1 << 23, 256, "x")

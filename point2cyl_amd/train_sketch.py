@@ -121,6 +121,16 @@ def main(argv=None):
         return _main(a, rank, world, dev)
 
 
+def make_optimizer(a, model, pn_encoder):
+    """train_Point2Cyl.py:298-311: the backbone's parameters and the sketch encoder's, each with its learning rate (the decoder is frozen)."""
+    groups = []
+    if a.is_pc_train:
+        groups.append({"params": list(model.parameters()), "lr": a.learning_rate})
+    if a.is_im_train:
+        groups.append({"params": list(pn_encoder.parameters()), "lr": step_lr(0.001, 1000, 0.5, 0)})
+    return optim.from_arguments(a, groups, heads=[*model.fc2.parameters(), *pn_encoder.fc.parameters()])
+
+
 def _main(a, rank, world, dev):
     K, S, N = a.K, a.num_sk_point, a.num_point
     torch.manual_seed(a.seed)
@@ -139,12 +149,7 @@ def _main(a, rank, world, dev):
     for m_ in (model, implicit_net, pn_encoder, loaded_pn_encoder):
         ddp.broadcast_module(m_)
     ddp.preflight([model, implicit_net, pn_encoder, loaded_pn_encoder], dev)      # world > 1: eager collective + identical replicas (raises otherwise)
-    groups = []
-    if a.is_pc_train:
-        groups.append({"params": list(model.parameters()), "lr": a.learning_rate})                           # :298-311
-    if a.is_im_train:
-        groups.append({"params": list(pn_encoder.parameters()), "lr": step_lr(0.001, 1000, 0.5, 0)})
-    opt = optim.from_arguments(a, groups, heads=list(model.fc2.parameters()))
+    opt = make_optimizer(a, model, pn_encoder)
     log = None
     if rank == 0:
         os.makedirs(a.logdir, exist_ok=True)

@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from point2cyl_amd import _lib, ops, optim
+from point2cyl_amd import _lib, backbone, ops, optim, sketch, train_sketch
 
 ONE = ctypes.c_void_p(16)              # a non-null, 16-byte aligned dummy: arguments are checked before anything is dereferenced
 
@@ -145,3 +145,19 @@ def test_newton_schulz_size_limits():
         with pytest.raises(ValueError, match="2\\^23"):
             ops.ns_check_size(r, c, "x")
     ops.ns_check_size(1 << 23, 256, "x")
+
+
+@pytest.mark.parametrize("pc,im", [(True, True), (True, False), (False, True)])
+def test_sketch_trainer_leaves_output_layers_to_adam(pc, im):
+    """--optimizer muon: the backbone's heads and the sketch encoder's output layer keep Adam's rule, and a schedule of their group reaches them."""
+    a = train_sketch.build_parser().parse_args(["--optimizer", "muon"])
+    a.is_pc_train, a.is_im_train = pc, im
+    model, enc = backbone.backbone(output_sizes=[3, 16]), sketch.PointNetEncoder(256, 2, with_normals=True)
+    o = train_sketch.make_optimizer(a, model, enc)
+    rule = {id(p): g["use_muon"] for g in o.param_groups for p in g["params"]}
+    heads = [p for on, m in ((pc, model.fc2), (im, enc.fc)) if on for p in m.parameters()]
+    assert heads and not any(rule[id(p)] for p in heads)
+    others = [p for on, m in ((pc, model), (im, enc)) if on for p in m.parameters() if not any(p is h for h in heads)]
+    assert all(rule[id(p)] for p in others) and len(rule) == len(heads) + len(others)
+    assert [(g["source"], g["use_muon"]) for g in o.param_groups] == [(k, m) for k in range(pc + im) for m in (True, False)]
+    assert [g["lr"] for g in o.param_groups] == [lr for on, lr in ((pc, a.learning_rate), (im, 0.001)) if on for _ in range(2)]

@@ -237,7 +237,7 @@ def _main(a, rank, world, dev):
         nb = int(t.item())
     if nb == 0:
         raise SystemExit("dataset shard (%d clouds) is smaller than one batch (%d)" % (len(data), B))
-    trainable = [p for g in groups for p in g["params"]]
+    trainable = [p for g in opt.param_groups for p in g["params"]]
     sync = ddp.FlatGradSync(trainable, world)
     sampler = NormalPerPoint(1.8, 0.01)                                                                       # :262-266
     gstep, best, old_lr = 0, np.inf, a.learning_rate

@@ -151,6 +151,7 @@ class Muon(Adam):
         hit = self._mats.get(gi)
         if hit is not None and hit[0] == key:
             return hit
+        self._check_group(group)                   # (its settings may have been changed since it was added)
         dev = ps[0].device
         recs = []
         for p in ps:

@@ -161,3 +161,19 @@ def test_sketch_trainer_leaves_output_layers_to_adam(pc, im):
     assert all(rule[id(p)] for p in others) and len(rule) == len(heads) + len(others)
     assert [(g["source"], g["use_muon"]) for g in o.param_groups] == [(k, m) for k in range(pc + im) for m in (True, False)]
     assert [g["lr"] for g in o.param_groups] == [lr for on, lr in ((pc, a.learning_rate), (im, 0.001)) if on for _ in range(2)]
+
+
+def test_settings_changed_after_construction_are_checked(monkeypatch):
+    monkeypatch.setattr(_lib, "require_device", lambda *t: None)
+    monkeypatch.setattr(_lib, "on", lambda d: _lib._HERE_ALREADY)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(optim, "stream", lambda: 0)
+    monkeypatch.setattr(optim, "call", lambda f, *a, **k: None)
+    p = torch.nn.Parameter(torch.zeros(5, 4))
+    p.grad = torch.ones(5, 4)
+    for key, bad in (("adjust", "spectrall"), ("ns_steps", 0), ("ns_coeffs", (9.0, 9.0, 9.0)), ("ns_steps", 12)):
+        o = optim.Muon([p])
+        o.step()
+        o.param_groups[0][key] = bad
+        with pytest.raises(ValueError):
+            o.step()

@@ -259,3 +259,20 @@ def test_newton_schulz_and_muon_on_very_long_matrices(shape, dtype):
         optim.Muon([p], lr=1.0, momentum=0.0, adjust="spectral").step()
         scale = max(1.0, shape[0] / shape[1]) ** 0.5
         assert (p.detach().double() + scale * want).norm().item() <= scale * bound
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_quantized_rows_by_what_they_stand_for(dtype):
+    """Without the kernel's own expression for the scale: within a unit of max / 127 (one rounding of 1 / 127 and one of the product), the largest element 127, and every element within half
+    a step (the quotients are rounded exactly)."""
+    from point2cyl_amd import ops
+    r = gen(39)
+    M, K = 4000, 200
+    mags = torch.logspace(-30 if dtype != torch.float16 else -3, 30 if dtype != torch.float16 else 3, M, device="cuda")[:, None]
+    x = (r(M, K).clamp(-5, 5) * torch.exp(r(M, 1)) * mags).to(dtype)
+    h = ops.quantize_rows(x)
+    v, s = x.double(), h.scale.double()
+    top = v.abs().amax(1)
+    assert ((s - top / 127.0).abs() <= 2.0 ** -23 * top / 127.0).all()
+    assert (h.q.abs().amax(1) == 127).all() and int(h.q.min()) >= -127
+    assert ((h.q.double() * s[:, None] - v).abs() <= 0.5 * s[:, None] * (1.0 + 2.0 ** -30)).all()

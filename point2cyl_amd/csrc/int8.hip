@@ -852,7 +852,7 @@ extern "C" int p2c_int8_linear_few(const void *x, int xdtype, long long ldx, con
                                    long long ldadd, int act, float beta, float thr, void *out, long long ldo, int dtype, int M, int N, int K, int Kp,
                                    void *stream)
 {
-    if (i8_shape_bad(M, K, Kp) || !p2c_int8_few_supported(M, K) || N < 1 || N > (1 << 20) || xdtype < 0 || xdtype > 2 || ldx < 0) return P2C_EINVAL;
+    if (i8_shape_bad(M, K, Kp) || !p2c_int8_few_supported(M, K) || Kp > 2048 || N < 1 || N > (1 << 20) || xdtype < 0 || xdtype > 2 || ldx < 0) return P2C_EINVAL;
     I8Epi e;
     const int rc = i8_epilogue(e, nullptr, sw, bias, add, ldadd, act, beta, thr, out, ldo, dtype, N);
     if (rc != P2C_OK) return rc;

@@ -177,3 +177,12 @@ def test_settings_changed_after_construction_are_checked(monkeypatch):
         o.param_groups[0][key] = bad
         with pytest.raises(ValueError):
             o.step()
+
+
+def test_few_rows_refuse_columns_that_do_not_fit_the_workgroup():
+    """The rows of a one-launch product lie in LDS, padded: K was checked, the padded width was not."""
+    L = _lib.lib()
+    few = lambda M, K, Kp: L.p2c_int8_linear_few(ONE, 0, 8, ONE, ONE, None, None, 0, 0, 1.0, 20.0, ONE, 8, 0, M, 8, K, Kp, None)  # noqa: E731
+    flo = lambda M, K, Kp: L.p2c_int8_linear_float(ONE, 0, 8, ONE, ONE, None, None, 0, 0, 1.0, 20.0, ONE, 8, 0, M, 8, K, Kp, ONE, None)  # noqa: E731
+    for f in (few, flo):
+        assert f(4, 8, 2112) == -1 and f(4, 2048, 1 << 20) == -1

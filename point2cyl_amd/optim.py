@@ -146,8 +146,10 @@ class Muon(Adam):
                     raise RuntimeError("point2cyl_amd.optim.Muon: take one step before capturing one (a parameter has no momentum yet)")
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
         lr, wd, adjust = float(group["lr"]), float(group["weight_decay"]), group["adjust"]
-        key = (lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"]),
-               *[(t.data_ptr(), t.shape, t.stride(), t.dtype) for p in ps for t in (p, p.grad, self.state[p]["momentum_buffer"])])
+        key = [lr, wd, adjust, group["ns_steps"], repr(group["ns_coeffs"])]
+        for p in ps:
+            d, m = p.grad, self.state[p]["momentum_buffer"]
+            key += (p.data_ptr(), p.shape, p.stride(), d.data_ptr(), d.shape, d.stride(), m.data_ptr(), m.shape)
         hit = self._mats.get(gi)
         if hit is not None and hit[0] == key:
             return hit

@@ -21,14 +21,23 @@ class Adam(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
         self._tables, self._captured = {}, []
 
+    def _key(self, ps):
+        """Every pointer and size a table holds (after load_state_dict, or anything else that replaces exp_avg / exp_avg_sq, a cached table would otherwise
+        keep pointing at the old, freed moment tensors, and after p.data = p.data[:k] at elements behind the parameter); None: there are no moments yet."""
+        key = []
+        try:
+            for p in ps:
+                st = self.state[p]
+                key += p.data_ptr(), p.numel(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
+        except KeyError:
+            return None
+        return key
+
     def _table(self, gi, ps):
-        # the key covers every pointer and size the table holds: after load_state_dict (or anything else that replaces exp_avg / exp_avg_sq) the
-        # cached table would otherwise keep pointing at the old, freed moment tensors, and after p.data = p.data[:k] at elements behind the parameter
-        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), *((st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if "exp_avg" in (st := self.state.get(p, ())) else (0, 0)))
-                    for p in ps)
+        key = self._key(ps)
         cached = self._tables.get(gi)
         capturing = ps[0].is_cuda and torch.cuda.is_current_stream_capturing()
-        if cached is not None and cached[0] == key:
+        if cached is not None and key is not None and cached[0] == key:
             if capturing and not any(cached is c for c in self._captured):
                 self._captured.append(cached)          # the graph's replays read this table, also after an eager step with other gradients has replaced it
             return cached
@@ -57,8 +66,7 @@ class Adam(torch.optim.Optimizer):
         tab = torch.tensor(rows, dtype=torch.int64).to(dev, non_blocking=True)
         nel = torch.tensor(numel, dtype=torch.int64).to(dev, non_blocking=True)
         chk = torch.tensor(chunks, dtype=torch.int32).to(dev, non_blocking=True)
-        key = tuple((p.data_ptr(), p.numel(), p.grad.data_ptr(), self.state[p]["exp_avg"].data_ptr(), self.state[p]["exp_avg_sq"].data_ptr()) for p in ps)
-        cached = (key, tab, nel, chk, len(chunks), ps)
+        cached = (self._key(ps), tab, nel, chk, len(chunks), ps)
         self._tables[gi] = cached
         return cached
 

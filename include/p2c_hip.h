@@ -571,7 +571,8 @@ int p2c_eval_metrics_f32(const float *heads, int ld, int xoff, int woff, const f
  * Orthogonalised updates (csrc/muon.hip).  For every matrix X_0 = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with
  * A = X X^T (of the smaller side); coeffs_host [steps][3] = a, b, c.  Descriptors are HOST memory and are read during the call only; their
  * pointers are device pointers.  Strides in elements; sides <= 2^23, rows * cols <= 2^31, batch <= 65536.  A matrix with no rows, columns or batch entries is skipped.
- *   p2c_newton_schulz: dst = result.  src and dst of `dtype` (0 fp32, 1 bf16, 2 fp16), arithmetic of 32-bit accuracy for all of them.  src may be dst.
+ *   p2c_newton_schulz: dst = result.  src and dst of `dtype` (0 fp32, 1 bf16, 2 fp16), arithmetic of 32-bit accuracy for all of them.  src may be dst with
+ *     the same strides.
  *   p2c_muon_step_f32 (fp32, batch = 1, mom [rows][cols] contiguous): mom = momentum mom + (1 - momentum) G;
  *     U = nesterov ? (1 - momentum) G + momentum mom : mom;  dst = decay dst - scale newton_schulz(U).
  * The coefficients have to keep every |X| below 3.8 and the polynomial below 15 from a start of 1, and the steps from any one to the last may amplify

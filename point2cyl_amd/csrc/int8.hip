@@ -213,7 +213,7 @@ __device__ __forceinline__ float i8_softplus2(float z, const I8Poly &k)
 // registers, the row scale is one number, and a row's maximum is an in-lane affair.
 // A k-tile is multiplied in two halves; the reads of the next half and the copies of a later k-tile are issued between the products of this one, because
 // instructions issue in order and a wave behind a queue of copies does not multiply.  16384 x 4096 x 4096: 299 us with copies, reads and products in turn,
-// 270 so = 2040 TOP/s (a large library product without scales, bias or rounding: 2130).
+// 270 so (20 calls out of idle; in a long run 236 = 2330 TOP/s, a large library product without scales, bias or rounding 2210).
 template <int BM, int BN, int WR, int WC, int NST>
 struct I8Tile {
     static constexpr int RB = 64, NW = WR * WC, STAGE = (BM + BN) * RB, TM = BM / WR / 32, TN = BN / WC / 32;
@@ -487,8 +487,9 @@ struct I8Requant {
 // 32-bit activations never leave the registers.  out [M][ldo] int8, columns behind N zero; so [M].  Softplus is computed in units of log2(e) / beta
 // (scale and bias carry the factor, the row's scale divides it out).  64 rows in four waves, two workgroups per CU; with many rows 128 in eight waves, one
 // workgroup per CU that goes from tile to tile (FLOW): the next tile's operands arrive during the epilogue, and the weights are read half as often.
-// 262144 x 512 x 512 with softplus: 191 us and 180.  Of the 191's clocks 30 % went with the copies (a tile of 64 rows reads all the weights: 1.2 GB through
-// the L2s), 12 % with the activation (17 vector instructions per element and an exponential in the whole epilogue), 10 % with the stores, 4 % with the products.
+// 262144 x 512 x 512 with softplus: 191 us and 180 in turn, from 20 calls out of idle; in a long run of calls the second takes 159.  Of the 191's clocks, by leaving out one part
+// at a time, 30 % went with the copies (a tile of 64 rows reads all the weights: 1.2 GB through the L2s), 12 % with the activation (17 vector instructions per
+// element and an exponential in the whole epilogue), 10 % with the stores, 4 % with the products; what the other 44 % go with is not known.
 template <int BM, int BN, int WR, int WC, int NST, bool FLOW, int ACT>
 __global__ void __launch_bounds__(64 * WR * WC, 2) int8_requant_kernel(const int8_t *__restrict__ x, const int8_t *__restrict__ w, long long ldx, int Kp,
                                                                        int M, int N, I8Epi e)
@@ -818,10 +819,9 @@ extern "C" int p2c_int8_linear(const int8_t *xq, long long ldx, const float *sx,
     if (((uintptr_t)xq & 15) || ((uintptr_t)wq & 15) || ldx % 16) return P2C_EALIGN;
     const hipStream_t st = (hipStream_t)stream;
     // 256 x 256 reads each operand half as often as 128 x 128 (16384 x 4096 x 4096: 270 us against 384; 262144 x 512 x 512: 142 against 153), but has to
-    // fill most of the 256 CUs; the same limit for 128 x 128 against 64 x 64.
-    // 256 x 256 reads each operand half as often as 128 x 128 (16384 x 4096 x 4096: 270 us against 384; 262144 x 512 x 512: 142 against 153), but has to
     // fill most of the 256 CUs; the same limit for 128 x 128 against 64 x 64.  From two tiles per CU on, one workgroup takes them one after the other
-    // (16384 x 4096 x 4096: 278 -> 267 us; k-tiles for all three stages needed).
+    // (16384 x 4096 x 4096: 278 -> 267 us; k-tiles for all three stages needed).  All of these from 20 calls out of idle, both forms in turn; in a long run of
+    // calls, at its clock, the product of 16384 x 4096 x 4096 takes 236 us = 2330 TOP/s and that of 262144 x 512 x 512 136.
     const long long t256 = (long long)p2c_cdiv(M, 256) * p2c_cdiv(N, 256);
     if (t256 >= 2 * I8_CUS && Kp >= 192) return linear_any<256, 256, 2, 4, 3, true>(xq, ldx, wq, Kp, M, N, e, st);
     if (t256 >= 192) return linear_any<256, 256, 2, 4, 3, false>(xq, ldx, wq, Kp, M, N, e, st);

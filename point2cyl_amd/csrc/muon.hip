@@ -322,8 +322,8 @@ __device__ __forceinline__ uint2 ns_quad_transpose(uint2 r, int lane)
 // 8 x 1024 x 2048: T' 136 us with reads, copies and products in turn, 123 with the reads a half ahead, 112 with the copies spread).
 // The addend b A, a T is the product's own first operand, so it is picked up when its block passes by: a product with the unit matrix, exact, into sums of
 // its own (into the product's it would be rounded again by every later step).  Fetched from memory in the results' layout it cost 10000 clocks a tile.
-// What bounds it at 8 x 1024 x 2048: the card's power.  T' runs 103 GFLOP in 115 us (900 TFLOP/s, against 1160 of a large library product) at 1.75 GHz;
-// the same launches on zeros take 24 us less.
+// What bounds it at 8 x 1024 x 2048: T' runs 103 GFLOP in 107 us (960 TFLOP/s; a large library product, under the same power limit, 1160 - 1220).  Power sets the clock
+// (1.75 GHz; the same launches on zeros take 24 us less); the rest of the distance has not been attributed.  A: 73 us for 576 tiles on 512 places, a second round for 64.
 template <int TR, int TB, int KG, int NST, int PH>
 __global__ void __launch_bounds__(64 * ns_waves(TB) * KG, 2) ns_product_kernel(const NsTab *__restrict__ tab, const NsRec *__restrict__ recs, const float ca, const float cb, const int cur)
 {
@@ -582,9 +582,10 @@ __device__ __forceinline__ void ns_put8(char *p, long long at, long long cs, int
 }
 
 // ---- matrices of up to 16384 elements (sides padded to 64: 128 x 128, 64 x 256): one workgroup each, all steps without leaving LDS.  The tiled form is
-// a chain of 17 launches of 4 us; here a step is three products of 1.5 us (both operands of a 128 x 128 product out of LDS: 384 KB, as long as its
-// matrix instructions).  S, then A, then B share one region: S is read by the first product only, and a X comes from the registers, which hold X in 32
-// bits in the layout of the products' results.  Measured at 128 x 128: 64 -> 50 us a call.
+// a chain of 17 launches of 4 us.  Here a call of 128 x 128 is 52 us (64 tiled): fifteen products of 3.4.  A product's matrix instructions and its operand reads
+// out of LDS (384 KB) take 1.3 - 1.5 us each and overlap; the rest lies between the products: six workgroup barriers a step, as S, then A, then B share one region
+// (S is read by the first product only, and a X comes from the registers, which hold X in 32 bits in the layout of the products' results), the splitting and storing of
+// every result, and A, which is read back for b A.
 constexpr int NS_MID = 16384;
 
 struct NsMidImage { int base, rows; };                          // offset in LDS; [k-tile][row][128 bytes], chunks permuted as in tile_dma.h
@@ -1044,7 +1045,7 @@ inline int ns_short(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.rows : 
 inline int ns_long(const p2c_ns_matrix &m) { return m.rows < m.cols ? m.cols : m.rows; }
 
 // ns_small takes 9 us for small sides up to 8 and 64 columns, 12 for 5 x 500, 15 for 16 x 64, 31 for 16 x 512, 97 for 12 x 2000; the other forms take 27, 62, 27, 63
-// and 82 (and on 32 rows, which ns_small could hold as well, 27 for 32 x 64 against 47, 82 for 32 x 2000 against 273).
+// and 82.
 inline bool ns_is_small(const p2c_ns_matrix &m) { return ns_short(m) <= 8 || (ns_short(m) <= NS_SMALL && ns_long(m) <= 1024); }
 
 // How a chunk is run.  Small matrices have a launch of their own - unless there are larger ones whose launches they can ride in: they lengthen none of their

@@ -113,8 +113,8 @@ class Muon(Adam):
         m <- momentum m + (1 - momentum) g;   u = (1 - momentum) g + momentum m with nesterov, else m
         p <- (1 - lr weight_decay) p - lr s newton_schulz(u)
     with s = 0.2 sqrt(max(rows, columns)) for adjust="rms" (an update of the size Adam's has: Adam's learning rates and schedules carry over) or
-    sqrt(max(1, rows / columns)) for "spectral".  All matrices of a parameter group go through csrc/muon.hip together: 17 launches whatever their
-    number (chunks of 24), momentum, norm, normalisation, decay and update included.  Vectors and scalars (biases, BatchNorm), and every parameter of a
+    sqrt(max(1, rows / columns)) for "spectral".  All matrices of a parameter group go through csrc/muon.hip together, 24 at a time: 17 launches
+    (one if they all fit a workgroup each), momentum, norm, normalisation, decay and update included.  Vectors and scalars (biases, BatchNorm), and every parameter of a
     group with use_muon=False, take Adam's rule with the group's `betas` and `adam_eps` in one launch, without decay.
 
     fp32, contiguous; `param_groups`, `state_dict` keep torch's shapes (state: "momentum_buffer" for matrices, Adam's three for the others).  A step can

@@ -276,3 +276,33 @@ def test_quantized_rows_by_what_they_stand_for(dtype):
     assert ((s - top / 127.0).abs() <= 2.0 ** -23 * top / 127.0).all()
     assert (h.q.abs().amax(1) == 127).all() and int(h.q.min()) >= -127
     assert ((h.q.double() * s[:, None] - v).abs() <= 0.5 * s[:, None] * (1.0 + 2.0 ** -30)).all()
+
+
+@pytest.mark.parametrize("kind", ["gauss", "lowrank", "decay"])
+@pytest.mark.parametrize("shapes,batch", [([(128, 128)], 0), ([(50, 256)], 0), ([(200, 1000)], 0), ([(1024, 512)], 0), ([(700, 500)], 12), ([(12, 400)], 0),
+                                          ([(8, 512), (16, 500), (3, 128), (512, 512)], 0), ([(8, 120), (60, 90), (1, 100)], 0)])
+def test_newton_schulz_is_as_exact_as_32_bits(shapes, batch, kind):
+    """Operands of 22 bits at least, products and sums of 32-bit size: at most four times (two bits) the error that plain 32-bit arithmetic makes of the same matrix, beside two units of
+    rounding of the result itself."""
+    from point2cyl_amd import ops
+    r = gen(40)
+
+    def make(m, n):
+        if kind == "lowrank":
+            k = max(1, min(m, n) // 16)
+            return r(m, k) @ r(k, n) / k ** 0.5 + 0.3 * r(m, n)
+        return r(m, n) * (torch.logspace(0, -3, m, device="cuda")[:, None] if kind == "decay" else 1.0)
+
+    def plain(G, dtype):
+        X = (G.double() / (G.double().norm() + 1e-7)).to(dtype)
+        X = X.t().contiguous() if G.shape[0] > G.shape[1] else X
+        for _ in range(5):
+            A = X @ X.t().contiguous()
+            X = NSC[0] * X + (NSC[1] * A + NSC[2] * (A @ A)) @ X
+        return X.t() if G.shape[0] > G.shape[1] else X
+    Gs = [make(*shapes[0]) for _ in range(batch)] if batch else [make(*s) for s in shapes]
+    os_ = list(ops.newton_schulz(torch.stack(Gs))) if batch else ops.newton_schulz(Gs)
+    for G, o in zip(Gs, os_):
+        want = plain(G, torch.float64)
+        err = lambda x: (x.double() - want).norm().item()  # noqa: E731
+        assert err(o) <= 4.0 * err(plain(G, torch.float32)) + 2.0 ** -22 * want.norm().item(), tuple(G.shape)

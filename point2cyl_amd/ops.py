@@ -1629,11 +1629,12 @@ def newton_schulz(G, steps=5, coeffs=NS_COEFFS, eps=1e-7):
             raise ValueError("newton_schulz: matrices on %s and %s in one call" % (dev, g.device))
         if g.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("newton_schulz has no gradient: call it under torch.no_grad() or on a detached tensor")
+        if g.numel():
+            ns_check_size(*g.shape[-2:], "newton_schulz")
         o = torch.empty(g.shape, dtype=g.dtype, device=dev)
         outs.append(o)
         if g.numel():
             src, dst = (g, o) if g.dim() == 2 else (g.reshape(-1, *g.shape[-2:]), o.view(-1, *g.shape[-2:]))
-            ns_check_size(*src.shape[-2:], "newton_schulz")
             # (bound to `src` until the launch: reshape may have made a copy)
             mine = groups.setdefault(_DTYPES[g.dtype], [])
             if src.dim() == 2:

@@ -306,3 +306,15 @@ def test_newton_schulz_is_as_exact_as_32_bits(shapes, batch, kind):
         want = plain(G, torch.float64)
         err = lambda x: (x.double() - want).norm().item()  # noqa: E731
         assert err(o) <= 4.0 * err(plain(G, torch.float32)) + 2.0 ** -22 * want.norm().item(), tuple(G.shape)
+
+
+def test_newton_schulz_refuses_large_matrices_before_it_allocates():
+    from point2cyl_amd import ops
+    one = torch.ones(1, 1, device="cuda")
+    before = torch.cuda.max_memory_allocated()
+    for shape in ((1 << 24, 1 << 16), ((1 << 23) + 1, 2), (1 << 32, 1), (1 << 16, (1 << 15) + 1)):
+        for G in (one.expand(*shape), one.expand(2, *shape), [one, one.expand(*shape)]):
+            with pytest.raises(ValueError, match="2\\^23"):
+                ops.newton_schulz(G)
+    assert torch.cuda.max_memory_allocated() < before + (1 << 20)
+    assert ops.newton_schulz(one.expand(1, 1)[:0].expand(0, 1 << 24)).shape == (0, 1 << 24)

@@ -393,6 +393,12 @@ class Int8ImplicitNet:
         M = input.shape[0]
         if M == 0:
             return torch.empty(0, self.last[3], dtype=torch.float32, device=input.device)
+        if input.device != self.first[0].device:
+            raise ValueError("Int8ImplicitNet: rows on %s, weights on %s" % (input.device, self.first[0].device))
+        with _lib.on(input.device):
+            return self._apply(input)
+
+    def _apply(self, input):
         inp = _c(F.pad(input, (0, (-self.d_in) % 4)) if self.d_in % 4 else input)
         sp = (self.beta, 20.0) if self.beta > 0 else None
         x = _prod_nt(inp, *self.first, sp=sp)

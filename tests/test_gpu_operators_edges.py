@@ -318,3 +318,30 @@ def test_newton_schulz_refuses_large_matrices_before_it_allocates():
                 ops.newton_schulz(G)
     assert torch.cuda.max_memory_allocated() < before + (1 << 20)
     assert ops.newton_schulz(one.expand(1, 1)[:0].expand(0, 1 << 24)).shape == (0, 1 << 24)
+
+
+def test_int8_decoder_runs_on_its_rows_device(monkeypatch):
+    """Every launch of the 8-bit decoder, the 32-bit ones among them, is made with the rows' device current; rows elsewhere than the weights are refused."""
+    from point2cyl_amd import _lib, implicit
+    net = implicit.ImplicitNet(d_in=6, dims=[64, 40, 48], skip_in=(2,), geometric_init=True, radius_init=1, beta=100).cuda()
+    q = implicit.Int8ImplicitNet(net)
+    x = gen(41)(300, 6)
+    want, inside, products, on, prod = q(x), [], [], _lib.on, implicit._prod_nt
+
+    class On:
+        def __init__(self, device):
+            self.device, self.real = device, on(device)
+
+        def __enter__(self):
+            inside.append(self.device)
+            self.real.__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return self.real.__exit__(*a)
+    monkeypatch.setattr(_lib, "on", On)
+    monkeypatch.setattr(implicit, "_prod_nt", lambda *a, **k: (products.append(list(inside)), prod(*a, **k))[1])
+    assert torch.equal(q(x), want) and len(products) == 3 and all(p == [x.device] for p in products)
+    q.first = tuple(t.cpu() for t in q.first)
+    with pytest.raises(ValueError, match="weights on"):
+        q(x)

@@ -345,3 +345,24 @@ def test_int8_decoder_runs_on_its_rows_device(monkeypatch):
     q.first = tuple(t.cpu() for t in q.first)
     with pytest.raises(ValueError, match="weights on"):
         q(x)
+
+
+def test_int8_products_of_rows_past_32_bit_offsets():
+    """2^26 + 700 rows of 64 bytes: the last ones lie beyond 2^32 bytes.  They are the numbers that a call on them alone gives (a row's sums are exact, its scaling its own)."""
+    from point2cyl_amd import ops
+    M, K, N = (1 << 26) + 700, 5, 6
+    r = gen(42)
+    x = r(M + K).as_strided((M, K), (1, 1))
+    w = ops.Int8Weight(r(N, K), r(N))
+    tail, mid = slice(M - 700, M), slice((1 << 25) - 300, (1 << 25) + 300)
+    y = ops.linear_int8(x, w, out_dtype=torch.bfloat16)
+    for part in (tail, mid):
+        assert torch.equal(y[part], ops.linear_int8(x[part], w, out_dtype=torch.bfloat16))
+    del y
+    h = ops.linear_int8(x, w, act="relu", requantize=True)
+    for part in (tail, mid):
+        p = ops.linear_int8(x[part], w, act="relu", requantize=True)
+        assert torch.equal(h.q[part], p.q) and torch.equal(h.scale[part], p.scale)
+    d = h.dequantize(torch.float16)
+    assert torch.equal(d[mid], p.dequantize(torch.float16))
+    assert torch.equal(d[tail], ops.linear_int8(x[tail], w, act="relu", requantize=True).dequantize(torch.float16))
